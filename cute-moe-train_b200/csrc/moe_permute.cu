@@ -1,0 +1,542 @@
+// Tokens sorted by expert and back (one GPU): the plan, the copies, the weighted sums and the gradients.
+//
+//   sort       stable counting sort of the n = tokens * topk routed copies (copy c = token * topk + slot) by
+//              expert; an id of -1 drops its copy.  offs[e] = end of expert e's rows, row_of_copy[c] = the
+//              copy's row or -1, copy_of_row[r] = the row's copy or -1 behind the last row.
+//   permute    rows[row_of_copy[c]] = x[c / topk]; rows behind the last one are zeros
+//   unpermute  out[t] = sum_j w[t, j] * rows[row_of_copy[t, j]]       (fp32 sum, one rounding; w absent: 1)
+//   gradients  of permute: unpermute without weights.  Of unpermute: drows[r] = w[c] * g[t] and
+//              dw[c] = <rows[r], g[t]> in one pass over the rows.
+//
+// Everything but the sort moves rows once and is bound by HBM: 16-byte accesses, each token's row is read
+// once and written to its topk rows (not gathered once per row), several accesses in flight per thread.
+// No atomics: every sum has a fixed order, so results repeat bit for bit.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "moe_gemm.h"
+
+namespace mgf {
+
+unsigned int* status_word_address();
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr unsigned kFull = 0xffffffffu;
+constexpr int kWarps = 8;  // warps per block of the row kernels
+
+// ---------------------------------------------------------------- sort
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortBatch = 4;  // ids loaded ahead per lane
+
+// One cluster of CTAs sorts all copies in one launch.  The copies are split into contiguous ranges, one
+// per warp; a warp ranks 32 copies at a time with match.any and keeps its own histogram in shared
+// memory, so the order within an expert is the copies' order.  Pass 1 counts, the histograms are
+// prefix-summed over the warps of a CTA, over the CTAs (distributed shared memory) and over the experts,
+// pass 2 walks the same ranges again and writes.
+__device__ __forceinline__ int load_id(const int64_t* ids, int64_t i, int64_t end, int E, bool& bad) {
+  if (i >= end) return -1;
+  const int64_t v = __ldg(ids + i);
+  if (v >= E || v < -1) {
+    bad = true;
+    return -1;
+  }
+  return static_cast<int>(v);
+}
+
+__global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
+                                                            int32_t* __restrict__ offs,
+                                                            int32_t* __restrict__ row_of_copy,
+                                                            int32_t* __restrict__ copy_of_row,
+                                                            unsigned int* __restrict__ status) {
+  extern __shared__ int32_t smem[];
+  int32_t* hist = smem;                     // [kSortWarps][E]
+  int32_t* total = smem + kSortWarps * E;   // [E] this CTA's counts, read by the other CTAs
+  int32_t* base = total + E;                // [E] first row of this CTA's copies of each expert
+  __shared__ int32_t warp_sums[kSortWarps];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t units = static_cast<int64_t>(ctas) * kSortWarps;
+  const int64_t per = ((n + units - 1) / units + 31) / 32 * 32;
+  const int64_t unit = static_cast<int64_t>(rank) * kSortWarps + warp;
+  const int64_t begin = unit * per < n ? unit * per : n;
+  const int64_t end = begin + per < n ? begin + per : n;
+  for (int i = threadIdx.x; i < kSortWarps * E; i += kSortThreads) hist[i] = 0;
+  __syncthreads();
+  int32_t* mine = hist + warp * E;
+  bool bad = false;
+  for (int64_t i = begin; i < end; i += 32 * kSortBatch) {
+    int id[kSortBatch];
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) id[b] = load_id(ids, i + 32 * b + lane, end, E, bad);
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      const unsigned same = __match_any_sync(kFull, id[b]);
+      if (id[b] >= 0 && lane == __ffs(same) - 1) mine[id[b]] += __popc(same);
+      __syncwarp();
+    }
+  }
+  if (__any_sync(kFull, bad) && lane == 0) atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += kSortThreads) {
+    int32_t run = 0;
+#pragma unroll 8
+    for (int w = 0; w < kSortWarps; ++w) {
+      const int32_t c = hist[w * E + e];
+      hist[w * E + e] = run;
+      run += c;
+    }
+    total[e] = run;
+  }
+  cluster.sync();
+  // one expert per thread (E <= 1024 = kSortThreads): counts of all CTAs and of those before this one
+  int32_t all = 0, before = 0;
+  if (threadIdx.x < E) {
+    for (int c = 0; c < ctas; ++c) {
+      const int32_t v = cluster.map_shared_rank(total, c)[threadIdx.x];
+      all += v;
+      before += c < rank ? v : 0;
+    }
+  }
+  int32_t incl = all;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int32_t o = __shfl_up_sync(kFull, incl, off);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  if (warp == 0) {
+    int32_t s = warp_sums[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int32_t o = __shfl_up_sync(kFull, s, off);
+      if (lane >= off) s += o;
+    }
+    warp_sums[lane] = s;
+  }
+  __syncthreads();
+  const int32_t first = incl - all + (warp > 0 ? warp_sums[warp - 1] : 0);
+  if (threadIdx.x < E) {
+    base[threadIdx.x] = first + before;
+    if (rank == 0) offs[threadIdx.x] = first + all;
+  }
+  const int32_t kept = warp_sums[kSortWarps - 1];
+  __syncthreads();
+  for (int64_t i = begin; i < end; i += 32 * kSortBatch) {
+    int id[kSortBatch];
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) id[b] = load_id(ids, i + 32 * b + lane, end, E, bad);
+#pragma unroll
+    for (int b = 0; b < kSortBatch; ++b) {
+      const int64_t c = i + 32 * b + lane;
+      const unsigned same = __match_any_sync(kFull, id[b]);
+      int32_t row = -1;
+      if (id[b] >= 0) row = base[id[b]] + mine[id[b]] + __popc(same & ((1u << lane) - 1u));
+      __syncwarp();
+      if (id[b] >= 0 && lane == __ffs(same) - 1) mine[id[b]] += __popc(same);
+      __syncwarp();
+      if (c < end) {
+        row_of_copy[c] = row;
+        if (row >= 0) copy_of_row[row] = static_cast<int32_t>(c);
+      }
+    }
+  }
+  for (int64_t r = kept + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n;
+       r += static_cast<int64_t>(ctas) * kSortThreads)
+    copy_of_row[r] = -1;
+  cluster.sync();  // no CTA leaves while another may still read its counts
+}
+
+// ---------------------------------------------------------------- row access
+// V elements of 16 bytes (VEC) or one element at a time where a base, a pitch or the width is not a
+// multiple of 16 bytes.
+template <typename T, bool VEC>
+struct Access {
+  static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
+  struct Raw {
+    T v[N];
+  };
+  static __device__ __forceinline__ Raw load(const T* p) {
+    Raw r;
+    if constexpr (VEC) {
+      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+      *reinterpret_cast<uint4*>(r.v) = u;
+    } else {
+      r.v[0] = __ldg(p);
+    }
+    return r;
+  }
+  static __device__ __forceinline__ void store(T* p, const Raw& r) {
+    if constexpr (VEC) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.v);
+    else p[0] = r.v[0];
+  }
+};
+
+__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f(float v) { return v; }
+__device__ __forceinline__ void put(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void put(__half& d, float v) { d = __float2half_rn(v); }
+__device__ __forceinline__ void put(float& d, float v) { d = v; }
+
+__device__ __forceinline__ bool row_ok(int32_t r, int64_t n_rows, unsigned int* status) {
+  if (r < 0) return false;  // dropped copy
+  if (r >= n_rows) {        // a wrong plan: report it, touch nothing
+    atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
+    return false;
+  }
+  return true;
+}
+
+// Zeros into the rows behind the last one, offs_end[0] .. n_rows, shared out over the whole grid.
+template <typename T, bool VEC>
+__device__ __forceinline__ void zero_tail(T* rows, int64_t ld, int64_t n_rows, int64_t nv, const int32_t* offs_end) {
+  int64_t kept = __ldg(offs_end);
+  if (kept < 0) kept = 0;
+  if (kept >= n_rows) return;
+  using A = Access<T, VEC>;
+  typename A::Raw z;
+#pragma unroll
+  for (int i = 0; i < A::N; ++i) put(z.v[i], 0.0f);
+  const int64_t w0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  const int64_t nw = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
+  for (int64_t r = kept + w0; r < n_rows; r += nw)
+    for (int64_t v = threadIdx.x & 31; v < nv; v += 32) A::store(rows + r * ld + v * A::N, z);
+}
+
+// ---------------------------------------------------------------- permute
+constexpr int kPermuteVecs = 4;  // vectors per lane and work unit: a warp moves 2 KB of one token
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps)
+    permute_kernel(const T* __restrict__ x, int64_t ldx, int64_t tokens, int topk, int64_t nv, int64_t chunks,
+                   const int32_t* __restrict__ row_of_copy, const int32_t* __restrict__ offs_end, int64_t n_rows,
+                   T* __restrict__ rows, int64_t ldr, unsigned int* __restrict__ status) {
+  using A = Access<T, VEC>;
+  const int lane = threadIdx.x & 31;
+  const int64_t u = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  if (u < tokens * chunks) {
+    const int64_t t = u / chunks;
+    const int64_t v0 = (u - t * chunks) * (32 * kPermuteVecs) + lane;
+    typename A::Raw r[kPermuteVecs];
+#pragma unroll
+    for (int i = 0; i < kPermuteVecs; ++i)
+      if (v0 + 32 * i < nv) r[i] = A::load(x + t * ldx + (v0 + 32 * i) * A::N);
+    for (int j = 0; j < topk; ++j) {
+      const int32_t row = __ldg(row_of_copy + t * topk + j);
+      if (!row_ok(row, n_rows, status)) continue;
+      T* d = rows + static_cast<int64_t>(row) * ldr;
+#pragma unroll
+      for (int i = 0; i < kPermuteVecs; ++i)
+        if (v0 + 32 * i < nv) A::store(d + (v0 + 32 * i) * A::N, r[i]);
+    }
+  }
+  zero_tail<T, VEC>(rows, ldr, n_rows, nv, offs_end);
+}
+
+// ---------------------------------------------------------------- unpermute
+constexpr int kSumVecs = 2;   // vectors per lane and work unit
+constexpr int kSumBatch = 4;  // copies whose loads are in flight together
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * kWarps)
+    unpermute_kernel(const T* __restrict__ rows, int64_t ldr, int64_t n_rows, int64_t tokens, int topk, int64_t nv,
+                     int64_t chunks, const int32_t* __restrict__ row_of_copy, const float* __restrict__ weights,
+                     T* __restrict__ out, int64_t ldo, unsigned int* __restrict__ status) {
+  using A = Access<T, VEC>;
+  const int lane = threadIdx.x & 31;
+  const int64_t u = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
+  if (u >= tokens * chunks) return;
+  const int64_t t = u / chunks;
+  const int64_t v0 = (u - t * chunks) * (32 * kSumVecs) + lane;
+  float acc[kSumVecs][A::N];
+#pragma unroll
+  for (int i = 0; i < kSumVecs; ++i)
+#pragma unroll
+    for (int c = 0; c < A::N; ++c) acc[i][c] = 0.0f;
+  for (int j0 = 0; j0 < topk; j0 += kSumBatch) {
+    int32_t row[kSumBatch];
+    float w[kSumBatch];
+    typename A::Raw r[kSumBatch][kSumVecs];
+#pragma unroll
+    for (int b = 0; b < kSumBatch; ++b) {
+      row[b] = j0 + b < topk ? __ldg(row_of_copy + t * topk + j0 + b) : -1;
+      w[b] = weights != nullptr && j0 + b < topk ? __ldg(weights + t * topk + j0 + b) : 1.0f;
+      if (!row_ok(row[b], n_rows, status)) row[b] = -1;
+    }
+#pragma unroll
+    for (int b = 0; b < kSumBatch; ++b)
+      if (row[b] >= 0) {
+#pragma unroll
+        for (int i = 0; i < kSumVecs; ++i)
+          if (v0 + 32 * i < nv) r[b][i] = A::load(rows + static_cast<int64_t>(row[b]) * ldr + (v0 + 32 * i) * A::N);
+      }
+#pragma unroll
+    for (int b = 0; b < kSumBatch; ++b)
+      if (row[b] >= 0) {
+#pragma unroll
+        for (int i = 0; i < kSumVecs; ++i)
+          if (v0 + 32 * i < nv) {
+#pragma unroll
+            for (int c = 0; c < A::N; ++c) acc[i][c] = fmaf(w[b], to_f(r[b][i].v[c]), acc[i][c]);
+          }
+      }
+  }
+#pragma unroll
+  for (int i = 0; i < kSumVecs; ++i)
+    if (v0 + 32 * i < nv) {
+      typename A::Raw o;
+#pragma unroll
+      for (int c = 0; c < A::N; ++c) put(o.v[c], acc[i][c]);
+      A::store(out + t * ldo + (v0 + 32 * i) * A::N, o);
+    }
+}
+
+// ---------------------------------------------------------------- unpermute, backward
+constexpr int kBwdBatch = 4;  // copies handled per walk over the token's row
+
+// WPT warps per token (1: many tokens, 8: few).  Each lane keeps the partial dot products of up to
+// kBwdBatch copies; they are summed over the lanes by shuffles and over the warps in a fixed order.
+template <typename T, bool VEC, int WPT>
+__global__ void __launch_bounds__(32 * kWarps)
+    unpermute_bwd_kernel(const T* __restrict__ g, int64_t ldg, const T* __restrict__ rows, int64_t ldr, int64_t n_rows,
+                         int64_t tokens, int topk, int64_t nv, const int32_t* __restrict__ row_of_copy,
+                         const int32_t* __restrict__ offs_end, const float* __restrict__ weights,
+                         T* __restrict__ grad_rows, int64_t ldgr, float* __restrict__ grad_weights,
+                         unsigned int* __restrict__ status) {
+  using A = Access<T, VEC>;
+  __shared__ float part[kWarps][kBwdBatch];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t t = (static_cast<int64_t>(blockIdx.x) * kWarps + warp) / WPT;  // uniform over a block for WPT = kWarps
+  const int sub = warp % WPT;
+  if (t < tokens) {
+    for (int j0 = 0; j0 < topk; j0 += kBwdBatch) {
+      int32_t row[kBwdBatch];
+      float w[kBwdBatch], dot[kBwdBatch];
+#pragma unroll
+      for (int b = 0; b < kBwdBatch; ++b) {
+        row[b] = j0 + b < topk ? __ldg(row_of_copy + t * topk + j0 + b) : -1;
+        if (!row_ok(row[b], n_rows, status)) row[b] = -1;
+        w[b] = weights != nullptr && j0 + b < topk ? __ldg(weights + t * topk + j0 + b) : 1.0f;
+        dot[b] = 0.0f;
+      }
+      for (int64_t v = sub * 32 + lane; v < nv; v += 32 * WPT) {
+        const typename A::Raw gv = A::load(g + t * ldg + v * A::N);
+        typename A::Raw rv[kBwdBatch];
+        if (grad_weights != nullptr) {
+#pragma unroll
+          for (int b = 0; b < kBwdBatch; ++b)
+            if (row[b] >= 0) rv[b] = A::load(rows + static_cast<int64_t>(row[b]) * ldr + v * A::N);
+        }
+#pragma unroll
+        for (int b = 0; b < kBwdBatch; ++b) {
+          if (row[b] < 0) continue;
+          if (grad_weights != nullptr) {
+#pragma unroll
+            for (int c = 0; c < A::N; ++c) dot[b] = fmaf(to_f(rv[b].v[c]), to_f(gv.v[c]), dot[b]);
+          }
+          if (grad_rows != nullptr) {
+            typename A::Raw o;
+#pragma unroll
+            for (int c = 0; c < A::N; ++c) put(o.v[c], w[b] * to_f(gv.v[c]));
+            A::store(grad_rows + static_cast<int64_t>(row[b]) * ldgr + v * A::N, o);
+          }
+        }
+      }
+      if (grad_weights == nullptr) continue;
+#pragma unroll
+      for (int b = 0; b < kBwdBatch; ++b) {
+#pragma unroll
+        for (int off = 16; off; off >>= 1) dot[b] += __shfl_xor_sync(kFull, dot[b], off);
+      }
+      if constexpr (WPT == 1) {
+        if (lane < kBwdBatch && j0 + lane < topk) {
+          float d = dot[0];
+#pragma unroll
+          for (int b = 1; b < kBwdBatch; ++b) d = lane == b ? dot[b] : d;
+          grad_weights[t * topk + j0 + lane] = d;
+        }
+      } else {
+        static_assert(WPT == kWarps, "one token per block");
+        if (lane == 0) {
+#pragma unroll
+          for (int b = 0; b < kBwdBatch; ++b) part[warp][b] = dot[b];
+        }
+        __syncthreads();
+        if (warp == 0 && lane < kBwdBatch && j0 + lane < topk) {
+          float d = 0.0f;
+          for (int i = 0; i < kWarps; ++i) d += part[i][lane];
+          grad_weights[t * topk + j0 + lane] = d;
+        }
+        __syncthreads();
+      }
+    }
+  }
+  if (grad_rows != nullptr) zero_tail<T, VEC>(grad_rows, ldgr, n_rows, nv, offs_end);
+}
+
+// ---------------------------------------------------------------- host
+int elem_size(int32_t dtype) { return dtype == MGF_DT_F32 ? 4 : 2; }
+
+bool vec_ok(const void* p, int64_t ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * size) % 16 == 0;
+}
+
+// Calls f(element, VEC) for the element type and whether all rows can be accessed 16 bytes at a time.
+template <typename F>
+int for_type(int32_t dtype, bool vec, F&& f) {
+  switch (dtype) {
+    case MGF_DT_BF16:
+      return vec ? f(__nv_bfloat16{}, std::true_type{}) : f(__nv_bfloat16{}, std::false_type{});
+    case MGF_DT_F16:
+      return vec ? f(__half{}, std::true_type{}) : f(__half{}, std::false_type{});
+    default:
+      return vec ? f(float{}, std::true_type{}) : f(float{}, std::false_type{});
+  }
+}
+
+bool row_args_ok(int32_t dtype, int64_t tokens, int32_t topk, int64_t hidden, int64_t n_rows) {
+  return dtype >= MGF_DT_BF16 && dtype <= MGF_DT_F32 && tokens >= 0 && topk >= 1 && hidden >= 0 && n_rows >= 0 &&
+         n_rows <= INT32_MAX && tokens <= INT32_MAX / topk;
+}
+
+int launched() { return cudaGetLastError() == cudaSuccess ? MGF_OK : MGF_ERR_CUDA; }
+
+// Blocks for `units` warps of work; false where a one-dimensional grid cannot hold them.
+bool grid_of(int64_t units, unsigned& grid) {
+  const int64_t b = (units + kWarps - 1) / kWarps;
+  if (b > INT32_MAX) return false;
+  grid = static_cast<unsigned>(b > 0 ? b : 1);
+  return true;
+}
+
+}  // namespace
+}  // namespace mgf
+
+extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int32_t* offs,
+                            int32_t* row_of_copy, int32_t* copy_of_row, void* stream) {
+  using namespace mgf;
+  if (n < 0 || n > INT32_MAX || num_experts < 1 || num_experts > 1024 || offs == nullptr)
+    return MGF_ERR_INVALID_ARGUMENT;
+  if (n > 0 && (expert_idx == nullptr || row_of_copy == nullptr || copy_of_row == nullptr))
+    return MGF_ERR_INVALID_ARGUMENT;
+  unsigned int* status = status_word_address();
+  if (status == nullptr) return MGF_ERR_CUDA;
+  const size_t smem = static_cast<size_t>(kSortWarps + 2) * num_experts * sizeof(int32_t);
+  if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           static_cast<int>((kSortWarps + 2) * 1024 * sizeof(int32_t))) != cudaSuccess)
+    return MGF_ERR_CUDA;
+  // one CTA up to four batches per warp, then 2, 4 and 8 (the portable cluster size)
+  const int64_t per_cta = static_cast<int64_t>(kSortThreads) * kSortBatch;
+  const unsigned ctas = n <= per_cta ? 1 : n <= 2 * per_cta ? 2 : n <= 4 * per_cta ? 4 : 8;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(kSortThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = ctas;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, sort_kernel, expert_idx, n, static_cast<int>(num_experts), offs, row_of_copy,
+                            copy_of_row, status) == cudaSuccess
+             ? MGF_OK
+             : MGF_ERR_CUDA;
+}
+
+extern "C" int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden,
+                               const int32_t* row_of_copy, const int32_t* offs_end, void* rows, int64_t ldr,
+                               int64_t n_rows, void* stream) {
+  using namespace mgf;
+  if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
+  if (n_rows == 0 || hidden == 0) return MGF_OK;
+  if (offs_end == nullptr || rows == nullptr || (tokens > 0 && (x == nullptr || row_of_copy == nullptr)))
+    return MGF_ERR_INVALID_ARGUMENT;
+  unsigned int* status = status_word_address();
+  if (status == nullptr) return MGF_ERR_CUDA;
+  const int es = elem_size(dtype);
+  const bool vec = (hidden * es) % 16 == 0 && vec_ok(x, ldx, es) && vec_ok(rows, ldr, es);
+  return for_type(dtype, vec, [&](auto e, auto v) {
+    using T = decltype(e);
+    constexpr bool VEC = decltype(v)::value;
+    const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 32 * kPermuteVecs - 1) / (32 * kPermuteVecs);
+    unsigned grid;
+    if (!grid_of(tokens * chunks, grid)) return static_cast<int>(MGF_ERR_INVALID_ARGUMENT);
+    permute_kernel<T, VEC><<<grid, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const T*>(x), ldx, tokens, topk, nv, chunks, row_of_copy, offs_end, n_rows, static_cast<T*>(rows),
+        ldr, status);
+    return launched();
+  });
+}
+
+extern "C" int mgf_moe_unpermute(const void* rows, int32_t dtype, int64_t ldr, int64_t n_rows, int64_t tokens,
+                                 int32_t topk, int64_t hidden, const int32_t* row_of_copy, const float* weights,
+                                 void* out, int64_t ldo, void* stream) {
+  using namespace mgf;
+  if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
+  if (tokens == 0 || hidden == 0) return MGF_OK;
+  if (out == nullptr || row_of_copy == nullptr || (n_rows > 0 && rows == nullptr)) return MGF_ERR_INVALID_ARGUMENT;
+  unsigned int* status = status_word_address();
+  if (status == nullptr) return MGF_ERR_CUDA;
+  const int es = elem_size(dtype);
+  const bool vec = (hidden * es) % 16 == 0 && vec_ok(rows, ldr, es) && vec_ok(out, ldo, es);
+  return for_type(dtype, vec, [&](auto e, auto v) {
+    using T = decltype(e);
+    constexpr bool VEC = decltype(v)::value;
+    const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 32 * kSumVecs - 1) / (32 * kSumVecs);
+    unsigned grid;
+    if (!grid_of(tokens * chunks, grid)) return static_cast<int>(MGF_ERR_INVALID_ARGUMENT);
+    unpermute_kernel<T, VEC><<<grid, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const T*>(rows), ldr, n_rows, tokens, topk, nv, chunks, row_of_copy, weights, static_cast<T*>(out),
+        ldo, status);
+    return launched();
+  });
+}
+
+extern "C" int mgf_moe_unpermute_bwd(const void* grad_out, int64_t ldg, const void* rows, int64_t ldr, int32_t dtype,
+                                     int64_t n_rows, int64_t tokens, int32_t topk, int64_t hidden,
+                                     const int32_t* row_of_copy, const int32_t* offs_end, const float* weights,
+                                     void* grad_rows, int64_t ldgr, float* grad_weights, void* stream) {
+  using namespace mgf;
+  if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
+  if (grad_rows == nullptr && grad_weights == nullptr) return MGF_OK;
+  if (tokens > 0 && (grad_out == nullptr || row_of_copy == nullptr)) return MGF_ERR_INVALID_ARGUMENT;
+  if (offs_end == nullptr || (n_rows > 0 && grad_weights != nullptr && rows == nullptr))
+    return MGF_ERR_INVALID_ARGUMENT;
+  if (tokens == 0 && n_rows == 0) return MGF_OK;
+  unsigned int* status = status_word_address();
+  if (status == nullptr) return MGF_ERR_CUDA;
+  const int es = elem_size(dtype);
+  const bool vec = (hidden * es) % 16 == 0 && vec_ok(grad_out, ldg, es) &&
+                   (grad_weights == nullptr || vec_ok(rows, ldr, es)) &&
+                   (grad_rows == nullptr || vec_ok(grad_rows, ldgr, es));
+  return for_type(dtype, vec, [&](auto e, auto v) {
+    using T = decltype(e);
+    constexpr bool VEC = decltype(v)::value;
+    const int64_t nv = hidden / Access<T, VEC>::N;
+    auto run = [&](auto wpt) {
+      constexpr int WPT = decltype(wpt)::value;
+      unsigned grid;
+      if (!grid_of(tokens * WPT, grid)) return static_cast<int>(MGF_ERR_INVALID_ARGUMENT);
+      unpermute_bwd_kernel<T, VEC, WPT><<<grid, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(
+          static_cast<const T*>(grad_out), ldg, static_cast<const T*>(rows), ldr, n_rows, tokens, topk, nv, row_of_copy,
+          offs_end, weights, static_cast<T*>(grad_rows), ldgr, grad_weights, status);
+      return launched();
+    };
+    // one warp per token as soon as that fills the 148 SMs' 64 warps twice
+    if (tokens >= 2 * 148 * 64) return run(std::integral_constant<int, 1>{});
+    return run(std::integral_constant<int, kWarps>{});
+  });
+}

@@ -249,6 +249,66 @@ int mgf_fp8_quantize_weights(const void* w, int64_t E, int64_t K, int64_t N, int
 int mgf_fp8_quantize_weights_both(const void* w, int64_t E, int64_t K, int64_t N, int64_t s_e, int64_t s_k, void* qa,
                                   int64_t ldqa, float* sa, void* qb, int64_t ldqb, float* sb, void* stream);
 
+/* ------------------------------------------------------------------ the MoE block around the products
+ * (no counterpart in the reference, whose path starts from rows already in expert order). */
+enum mgf_dtype { MGF_DT_BF16 = 0, MGF_DT_F16 = 1, MGF_DT_F32 = 2 };
+enum mgf_route_score { MGF_ROUTE_SOFTMAX = 0, MGF_ROUTE_SIGMOID = 1 };
+
+/* Router.  logits [tokens, E] (E <= 1024, topk <= min(E, 32), row stride ld): the topk experts with the
+ * largest logit + bias (bias fp32 [E] or NULL, selection only), largest first, ties to the lowest expert.
+ * weights fp32 [tokens, topk]: scale * softmax (over the chosen experts if renormalize, else over all) or
+ * scale * sigmoid (divided by the chosen experts' sum if renormalize) of the logits without bias.
+ * expert_idx int64 [tokens, topk].  A logit or logit + bias of -inf is never chosen: slots left over, and
+ * all slots of tokens whose token_mask (bytes, or NULL) is 0, get id -1 and weight 0.
+ * mgf_moe_route_bwd: grad_logits [tokens, E] (row stride ldg, every element written) from the gradient of
+ * the weights; the chosen experts are those of expert_idx. */
+int mgf_moe_route(const void* logits, int32_t dtype, int64_t ld, int64_t tokens, int32_t num_experts, int32_t topk,
+                  int32_t score, int32_t renormalize, float scale, const float* bias, const uint8_t* token_mask,
+                  float* weights, int64_t* expert_idx, void* stream);
+int mgf_moe_route_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t tokens, int32_t num_experts, int32_t topk,
+                      int32_t score, int32_t renormalize, float scale, const int64_t* expert_idx,
+                      const float* grad_weights, void* grad_logits, int64_t ldg, void* stream);
+
+/* Plan of the permutation: stable counting sort of n routed copies (expert_idx int64 [n], copy c = token
+ * c / topk) by expert, E <= 1024.  offs int32 [E] (cumulative row ends, what the grouped products take),
+ * row_of_copy int32 [n] (-1 for a copy whose id is -1), copy_of_row int32 [n] (-1 behind offs[E-1]).  Ids
+ * outside [-1, E) drop their copy too and set MGF_DEV_ROW_OUT_OF_RANGE.  One launch. */
+int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int32_t* offs, int32_t* row_of_copy,
+                 int32_t* copy_of_row, void* stream);
+
+/* Rows by a plan (any hidden size; strides in elements; 16-byte accesses where every base and pitch and the
+ * width allow).  offs_end points at offs[E-1].  A row index >= n_rows is skipped and sets
+ * MGF_DEV_ROW_OUT_OF_RANGE.
+ *   permute:       rows[row_of_copy[t*topk+j]] = x[t]; rows from *offs_end to n_rows become zeros
+ *   unpermute:     out[t] = sum_j weights[t*topk+j] * rows[row_of_copy[t*topk+j]]  (fp32 sum; NULL weights: 1)
+ *   unpermute_bwd: grad_rows[row] = weight * grad_out[t] (rows behind *offs_end: zeros) and
+ *                  grad_weights[t*topk+j] = <rows[row], grad_out[t]> (0 for a dropped copy); either may be NULL. */
+int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden,
+                    const int32_t* row_of_copy, const int32_t* offs_end, void* rows, int64_t ldr, int64_t n_rows,
+                    void* stream);
+int mgf_moe_unpermute(const void* rows, int32_t dtype, int64_t ldr, int64_t n_rows, int64_t tokens, int32_t topk,
+                      int64_t hidden, const int32_t* row_of_copy, const float* weights, void* out, int64_t ldo,
+                      void* stream);
+int mgf_moe_unpermute_bwd(const void* grad_out, int64_t ldg, const void* rows, int64_t ldr, int32_t dtype,
+                          int64_t n_rows, int64_t tokens, int32_t topk, int64_t hidden, const int32_t* row_of_copy,
+                          const int32_t* offs_end, const float* weights, void* grad_rows, int64_t ldgr,
+                          float* grad_weights, void* stream);
+
+/* e4m3 quantisers with a scale per block of 128: bf16 in, float8_e4m3fn codes and fp32 scales out; the scale
+ * is the smallest power of two with amax / scale <= 448 (1 for a block of zeros, never subnormal), amax over
+ * the block's finite elements; non-finite elements become NaN codes.
+ *   rows:    x [tokens, cols] -> q (row stride ldq, a multiple of 16), scale [.., ceil(cols / 128)] (row
+ *            stride lds).  row_of_copy NULL: row t of q is token t (topk 1, n_rows = tokens).  Else the
+ *            token's codes go to its topk rows, and rows from *offs_end to n_rows get zero codes and scales.
+ *   weights: w [E, R, C] with unit stride along C -> q in the same layout (strides q_e, q_r multiples of 8)
+ *            and scale [E, ceil(R / 128), ceil(C / 128)] with any strides. */
+int mgf_fp8_block_quantize_rows(const void* x, int64_t ldx, int64_t tokens, int64_t cols, int32_t topk,
+                                const int32_t* row_of_copy, const int32_t* offs_end, void* q, int64_t ldq,
+                                float* scale, int64_t lds, int64_t n_rows, void* stream);
+int mgf_fp8_block_quantize_weights(const void* w, int64_t E, int64_t R, int64_t C, int64_t s_e, int64_t s_r, void* q,
+                                   int64_t q_e, int64_t q_r, float* scale, int64_t ss_e, int64_t ss_r, int64_t ss_c,
+                                   void* stream);
+
 /* Map a peer process's device allocation (its 64-byte cudaIpcMemHandle_t) into the context of
  * the calling thread's current device, peer access enabled, for mgf_push_rows destinations
  * (no counterpart in the reference).  mgf_ipc_close unmaps it. */
