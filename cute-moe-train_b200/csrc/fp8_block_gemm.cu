@@ -1,0 +1,655 @@
+// Grouped e4m3 GEMM with a scale for each block of 128 (ragged M), three fused epilogues.
+//
+//   acc[r, c] = sum over blocks b of 128 along k:  sa[r, b] * sb[e, b, c / 128] * (A[r, b] . B[e, b, c])
+//   MGF_EPI_BIAS        D = bf16(acc + bias[e])
+//   MGF_EPI_SWIGLU      aux = bf16(acc + bias[e]), D2 = clamped SwiGLU(aux)
+//   MGF_EPI_SWIGLU_BWD  D = SwiGLU_bwd(acc, aux)
+//
+// The scales change every 128 elements of k, so the tensor cores cannot keep one accumulator over the whole
+// contraction: each block's product goes into one of two TMEM buffers (4 tcgen05.mma of K = 32), and the
+// epilogue warps add it, scaled, to fp32 accumulators in registers while the next block is multiplied into
+// the other buffer.  A thread owns one row and 128 columns (one scale block) of the 128 x 256 tile, so the
+// factor sa * sb is one scalar per thread and block and the promotion is one FMA per element.  The two
+// sides balance: a block's MMAs take 512 clocks at the e4m3 rate, reading 128 x 256 fp32 from TMEM and adding
+// them 256 of the 512.
+//
+// B is read as stored, [E, k, n] with unit stride along n (the weights' own layout: MN-major operand) or along
+// k (the transposed view, the input gradient), so one set of codes serves both.  Warp roles, CTA pairs,
+// tile order, bounded waits and the handling of malformed offs are those of moe_gemm_sm100.cu.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+#include <cstdio>
+#include <cstdlib>
+#include <mutex>
+
+#include "epilogue.cuh"
+#include "host.h"
+#include "moe_gemm.h"
+#include "ptx.cuh"
+
+namespace mgf {
+namespace block_gemm {
+
+constexpr int BM = 128;             // rows of A per CTA
+constexpr int BK = 128;             // elements (= bytes) of k per stage = one scale block
+constexpr int kMaxGroups = 1024;
+constexpr int kNumEpiWarps = 8;     // two warpgroups, each half of the tile's columns
+constexpr int kThreads = 64 + 32 * kNumEpiWarps;
+constexpr uint64_t kWaitLimitNs = 1500ull * 1000ull * 1000ull;  // 1.5 s per pipeline wait
+constexpr uint64_t kDrainLimitNs = 100ull * 1000ull * 1000ull;
+
+template <int BN, int CG>
+struct Cfg {
+  static constexpr int A_BYTES = BM * BK;
+  static constexpr int BNC = BN / CG;  // columns of B held by this CTA
+  static constexpr int B_BYTES = BNC * BK;
+  static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SCHED_BYTES = 3 * 4 * (kMaxGroups + 1);
+  static constexpr int TAIL_BYTES = (BAR_BYTES + SCHED_BYTES + 1023) / 1024 * 1024;
+  static constexpr int BUDGET = 227 * 1024 - 1024 - TAIL_BYTES;
+  static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
+  static constexpr int TMEM_COLS = 2 * BN;
+  static_assert(STAGES >= 3 && (2 * STAGES + 5) * 8 + 8 <= BAR_BYTES && SMEM_BYTES <= 227 * 1024, "shared memory");
+};
+
+struct Params {
+  int E, n, k, n_tiles;
+  int64_t total_rows;
+  const int32_t* offs;
+  const float* scale_a;
+  int64_t lds_a;
+  const float* scale_b;
+  int64_t sb_e, sb_k, sb_n;
+  const __nv_bfloat16* bias;
+  int64_t bias_stride;
+  __nv_bfloat16* d;
+  int64_t ldd;
+  __nv_bfloat16* d2;
+  int64_t ldd2;
+  const __nv_bfloat16* aux;
+  int64_t ld_aux;
+  float alpha, limit;
+  int aux_v8, d_v8, d2_v8;  // base 32-byte aligned and row pitch a multiple of 32 bytes
+  int stall_test;           // test hook: no tile is loaded, so every consumer wait runs out
+  unsigned int* status;
+};
+
+struct Tile {
+  int e, n0, row0, row_end;
+};
+
+template <bool CLUSTER>
+__device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
+  if constexpr (CLUSTER) return ptx::mbar_try_wait_cluster(bar, parity);
+  return ptx::mbar_try_wait(bar, parity);
+}
+
+// Wait for phase `parity` of an mbarrier for at most `limit_ns`; CLUSTER acquires at cluster scope.
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                             unsigned int* status, uint64_t limit_ns = kWaitLimitNs) {
+  if (try_wait<CLUSTER>(bar, parity)) return true;
+  const uint64_t t0 = ptx::globaltimer_ns();
+  uint32_t it = 0;
+  while (true) {
+    if (try_wait<CLUSTER>(bar, parity)) return true;
+    if ((++it & 127u) == 0) {
+      if (*abort_flag) return false;
+      if (ptx::globaltimer_ns() - t0 > limit_ns) {
+        *abort_flag = 1;
+        atomicOr(status, MGF_DEV_WAIT_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// Group bounds clamped into [0, total_rows] and the prefix of their tile counts; one warp.
+template <int TM>
+__device__ void build_schedule(const Params& p, int* prefix, int* seg_start, int* seg_end, int lane) {
+  int running = 0;
+  bool bad = false;
+  const long long tr = p.total_rows;
+  for (int base = 0; base < p.E; base += 32) {
+    const int e = base + lane;
+    int cnt = 0;
+    if (e < p.E) {
+      const long long raw_prev = e == 0 ? 0 : (long long)__ldg(p.offs + e - 1);
+      const long long raw_end = (long long)__ldg(p.offs + e);
+      if (raw_end < raw_prev || raw_end > tr || raw_prev < 0) bad = true;
+      const long long sp = raw_prev < 0 ? 0 : (raw_prev > tr ? tr : raw_prev);
+      const long long ep = raw_end < sp ? sp : (raw_end > tr ? tr : raw_end);
+      seg_start[e] = (int)sp;
+      seg_end[e] = (int)ep;
+      cnt = (int)((ep - sp + TM - 1) / TM) * p.n_tiles;
+    }
+    int inc = cnt;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, inc, off);
+      if (lane >= off) inc += o;
+    }
+    if (e < p.E) prefix[e + 1] = running + inc;
+    running += __shfl_sync(0xffffffffu, inc, 31);
+  }
+  if (lane == 0) prefix[0] = 0;
+  if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(p.status, MGF_DEV_BAD_OFFS);
+}
+
+// Tile t: n fastest, so the CTAs at work share a few row blocks and the expert's weight slab.
+template <int TM, int BN>
+__device__ __forceinline__ Tile decode_tile(int t, const Params& p, const int* prefix, const int* seg_start,
+                                            const int* seg_end) {
+  int lo = 0, hi = p.E;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= t) lo = mid; else hi = mid;
+  }
+  const int local = t - prefix[lo], m_blk = local / p.n_tiles;
+  return Tile{lo, (local - m_blk * p.n_tiles) * BN, seg_start[lo] + m_blk * TM, seg_end[lo]};
+}
+
+// 16 consecutive fp32 columns of this thread's TMEM lane; no wait.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Sigmoid from the exponential (relative error a few 2^-23): the tanh form's absolute error of about 2^-12
+// would be a relative error of tens of percent at gates of -4.
+__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+
+__device__ __forceinline__ float swiglu(float g, float u, float alpha, float limit) {
+  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
+  return gc * sigmoid(alpha * gc) * (uc + 1.0f);
+}
+__device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, float alpha, float limit) {
+  const float g = bf16_lo(aux_word), u = bf16_hi(aux_word);
+  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
+  const float sig = sigmoid(alpha * gc);
+  const float d_gate = (g <= limit) ? gs * (uc + 1.0f) * sig * (1.0f + alpha * gc * (1.0f - sig)) : 0.0f;
+  const float d_up = (u >= -limit && u <= limit) ? gs * gc * sig : 0.0f;
+  return pack_bf16x2(d_gate, d_up);
+}
+
+template <int BN, int EPI, bool B_MN, int CG>
+__global__ void __launch_bounds__(kThreads, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+  using C = Cfg<BN, CG>;
+  constexpr int STAGES = C::STAGES;
+  constexpr int TM = BM * CG;       // rows of a tile
+  constexpr int COLS = BN / 2;      // columns of a tile that one epilogue thread owns
+  constexpr int kMmas = BK / 32;
+  static_assert(COLS == 128 || (COLS == 64 && CG == 1), "a thread's columns lie in one scale block");
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * C::STAGE_BYTES);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + STAGES;
+  uint64_t* tfull_bar = bars + 2 * STAGES;
+  uint64_t* tempty_bar = bars + 2 * STAGES + 2;
+  uint64_t* drain_bar = bars + 2 * STAGES + 4;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int* prefix = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES + C::BAR_BYTES);
+  int* seg_start = prefix + (kMaxGroups + 1);
+  int* seg_end = seg_start + (kMaxGroups + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = CG == 2 ? ptx::cluster_ctarank() : 0u;
+  const bool leader = crank == 0;
+  const int unit = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_units = CG == 2 ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(ptx::smem_u32(&tfull_bar[b]), 1);
+      ptx::mbar_init(ptx::smem_u32(&tempty_bar[b]), kNumEpiWarps * CG);
+    }
+    ptx::mbar_init(ptx::smem_u32(drain_bar), 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmA);
+    ptx::prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    if constexpr (CG == 2) {
+      ptx::tmem_alloc_pair(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
+      ptx::tmem_relinquish();
+    }
+  }
+  if (warp == 2) build_schedule<TM>(p, prefix, seg_start, seg_end, lane);
+  ptx::tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) ptx::cluster_sync();  // barriers of both CTAs initialised before any remote use
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int total_tiles = prefix[p.E];
+  const int nk = (p.k + BK - 1) / BK;
+
+  auto leader_addr = [&](const void* ptr) -> uint32_t {
+    const uint32_t a = ptx::smem_u32(ptr);
+    if constexpr (CG == 2) return ptx::mapa_shared(a, 0);
+    return a;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      uint32_t issued_parity[STAGES];
+      bool outstanding[STAGES];
+#pragma unroll
+      for (int s = 0; s < STAGES; ++s) { outstanding[s] = false; issued_parity[s] = 0; }
+      bool ok = true;
+      for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+        const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
+        const int nb0 = ti.n0 + static_cast<int>(crank) * C::BNC;
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!wait_bounded(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status)) { ok = false; break; }
+          uint32_t fb = ptx::smem_u32(&full_bar[stage]);
+          if constexpr (CG == 2) {  // both CTAs' bytes count on the even CTA's barrier
+            if (leader) ptx::mbar_arrive_expect_tx(fb, 2 * C::STAGE_BYTES);
+            else fb = leader_addr(&full_bar[stage]);
+          } else {
+            ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+          }
+          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + C::A_BYTES;
+          const int row = ti.row0 + static_cast<int>(crank) * BM;
+          if constexpr (CG == 2) {
+            ptx::tma_load_2d_pair(sA, &tmA, fb, kb * BK, row);
+            if constexpr (B_MN) ptx::tma_load_3d_pair(sB, &tmB, fb, nb0, kb * BK, ti.e);
+            else ptx::tma_load_3d_pair(sB, &tmB, fb, kb * BK, nb0, ti.e);
+          } else {
+            ptx::tma_load_2d(sA, &tmA, fb, kb * BK, row);
+            if constexpr (B_MN) {
+#pragma unroll
+              for (int c = 0; c < C::BNC / 128; ++c)
+                ptx::tma_load_3d(sB + c * 16384, &tmB, fb, nb0 + 128 * c, kb * BK, ti.e);
+            } else {
+              ptx::tma_load_3d(sB, &tmB, fb, kb * BK, nb0, ti.e);
+            }
+          }
+          outstanding[stage] = true;
+          issued_parity[stage] = phase;
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok && CG == 1) {
+        // Stopped early: let the copies in flight land before the CTA exits (a pair meets at its barrier).
+        for (int s = 0; s < STAGES; ++s)
+          if (outstanding[s])
+            wait_bounded(ptx::smem_u32(&full_bar[s]), issued_parity[s], abort_flag, p.status, kDrainLimitNs);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ UMMA issuer (even CTA)
+    constexpr uint32_t idesc = ptx::make_idesc_e4m3(BM * CG, BN, false, B_MN);
+    // MN-major B: 128-column chunks of 128 k rows, 16 KB apart, 32 k rows of 128 bytes per instruction;
+    // K-major: 32 bytes of every 128-byte row per instruction
+    constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
+    constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
+    constexpr uint32_t a_kstep = 32u >> 4;
+    uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, alternating TMEM buffers
+    bool ok = true, issued_any = false;
+    if (leader) {
+      for (int t = unit; ok && t < total_tiles; t += num_units) {
+        for (int kb = 0; kb < nk; ++kb, ++part) {
+          const uint32_t buf = part & 1, bph = (part >> 1) & 1;
+          ok = __all_sync(0xffffffffu, wait_bounded<CG == 2>(ptx::smem_u32(&tempty_bar[buf]), bph ^ 1, abort_flag, p.status));
+          if (!ok) break;
+          ok = __all_sync(0xffffffffu, wait_bounded<CG == 2>(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status));
+          if (!ok) break;
+          ptx::tc_fence_after();
+          if (lane == 0) {
+            const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+            const uint64_t adesc = ptx::make_smem_desc_sw128(sA, 16, 1024);
+            const uint64_t bdesc = ptx::make_smem_desc_sw128(sA + C::A_BYTES, b_lbo, 1024);
+            const uint32_t d_tmem = tmem_base + buf * BN;
+#pragma unroll
+            for (int kk = 0; kk < kMmas; ++kk) {
+              if constexpr (CG == 2) ptx::umma_f8_pair(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
+              else ptx::umma_f8(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
+            }
+            if constexpr (CG == 2) {
+              ptx::umma_commit_pair(ptx::smem_u32(&empty_bar[stage]), 0x3);
+              ptx::umma_commit_pair(ptx::smem_u32(&tfull_bar[buf]), 0x3);
+            } else {
+              ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
+              ptx::umma_commit(ptx::smem_u32(&tfull_bar[buf]));
+            }
+            issued_any = true;
+          }
+          __syncwarp();
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok && lane == 0 && issued_any) {
+        // Stopped early: wait for the UMMAs already issued before TMEM is released.
+        if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
+        else ptx::umma_commit(ptx::smem_u32(drain_bar));
+        wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, p.status, kDrainLimitNs);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ promotion and epilogue
+    const int q = warp & 3, wg = (warp - 2) >> 2;
+    const int r = q * 32 + lane;
+    const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + wg * COLS;
+    const uint32_t tempty_leader[2] = {leader_addr(&tempty_bar[0]), leader_addr(&tempty_bar[1])};
+    uint32_t part = 0;
+    bool ok = true;
+    for (int t = unit; ok && t < total_tiles; t += num_units) {
+      const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
+      const int c0 = ti.n0 + wg * COLS;                            // this thread's first column
+      const int crow0 = ti.row0 + static_cast<int>(crank) * BM;    // first row of this CTA's half
+      const int grow = crow0 + r;
+      const bool active = crow0 + q * 32 < ti.row_end && c0 < p.n;  // warp-uniform
+      const bool valid = grow < ti.row_end;
+      float acc[COLS];
+#pragma unroll
+      for (int j = 0; j < COLS; ++j) acc[j] = 0.0f;
+      // scales: this row's, one block ahead; the tile column block's, one block ahead
+      const float* sa_row = p.scale_a + (valid ? grow : ti.row0) * p.lds_a;
+      const float* sb_col = p.scale_b + ti.e * p.sb_e + (c0 / BK) * p.sb_n;
+      float sa = active ? __ldg(sa_row) : 0.0f, sb = active ? __ldg(sb_col) : 0.0f;
+      for (int kb = 0; kb < nk; ++kb, ++part) {
+        const uint32_t buf = part & 1, bph = (part >> 1) & 1;
+        const float s = sa * sb;
+        if (active && kb + 1 < nk) {
+          sa = __ldg(sa_row + kb + 1);
+          sb = __ldg(sb_col + (kb + 1) * p.sb_k);
+        }
+        ok = __all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(&tfull_bar[buf]), bph, abort_flag, p.status));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        if (active) {
+          const uint32_t tb = lane_base + buf * BN;
+          uint32_t v[2][16];
+          tmem_ld_x16(tb, v[0]);
+#pragma unroll
+          for (int c = 0; c < COLS / 16; ++c) {
+            ptx::tmem_ld_wait();
+            if (c + 1 < COLS / 16) tmem_ld_x16(tb + (c + 1) * 16, v[(c + 1) & 1]);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[c * 16 + j] = fmaf(s, __uint_as_float(v[c & 1][j]), acc[c * 16 + j]);
+          }
+        }
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) ptx::mbar_arrive_cluster(tempty_leader[buf]);
+          else ptx::mbar_arrive(ptx::smem_u32(&tempty_bar[buf]));
+        }
+      }
+      if (!ok) break;
+      if (!valid || !active) continue;
+      // 32 columns at a time; n is a multiple of 8 (SWIGLU: 16), so units of 8 columns are whole
+#pragma unroll
+      for (int c = 0; c < COLS / 32; ++c) {
+        const int col0 = c0 + c * 32;
+        if (col0 >= p.n) break;
+        if constexpr (EPI == MGF_EPI_SWIGLU_BWD) {
+          uint4 aw[8];
+          load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0, p.n, true, p.aux_v8, aw);
+          uint4* gp = reinterpret_cast<uint4*>(p.d + (int64_t)grow * p.ldd + 2 * col0);
+          const int nvalid = (p.n - col0) >> 2;
+#pragma unroll
+          for (int g = 0; g < 8; g += 2) {
+            if (g < nvalid) {
+              uint4 o[2];
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const float* f = acc + c * 32 + 4 * (g + h);
+                o[h].x = swiglu_bwd(f[0], aw[g + h].x, p.alpha, p.limit);
+                o[h].y = swiglu_bwd(f[1], aw[g + h].y, p.alpha, p.limit);
+                o[h].z = swiglu_bwd(f[2], aw[g + h].z, p.alpha, p.limit);
+                o[h].w = swiglu_bwd(f[3], aw[g + h].w, p.alpha, p.limit);
+              }
+              if (p.d_v8) ptx::st_v8(gp + g, o[0], o[1]);
+              else {
+                gp[g] = o[0];
+                gp[g + 1] = o[1];
+              }
+            }
+          }
+        } else {
+          uint32_t packed[16];
+          const uint4* bp = reinterpret_cast<const uint4*>(p.bias + (int64_t)ti.e * p.bias_stride + col0);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint4 b = make_uint4(0, 0, 0, 0);
+            if (p.bias != nullptr && col0 + 8 * g < p.n) b = __ldg(bp + g);
+            const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const float* f = acc + c * 32 + 8 * g + 2 * h;
+              packed[4 * g + h] = pack_bf16x2(f[0] + bf16_lo(w[h]), f[1] + bf16_hi(w[h]));
+            }
+          }
+          uint4 u[4];
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            u[g] = make_uint4(packed[4 * g], packed[4 * g + 1], packed[4 * g + 2], packed[4 * g + 3]);
+          store_units<4>(p.d + (int64_t)grow * p.ldd + col0, u, (p.n - col0) >> 3, p.d_v8);
+          if constexpr (EPI == MGF_EPI_SWIGLU) {
+            uint32_t so[8];
+#pragma unroll
+            for (int h = 0; h < 8; ++h)
+              so[h] = pack_bf16x2(
+                  swiglu(bf16_lo(packed[2 * h]), bf16_hi(packed[2 * h]), p.alpha, p.limit),
+                  swiglu(bf16_lo(packed[2 * h + 1]), bf16_hi(packed[2 * h + 1]), p.alpha, p.limit));
+            const uint4 us[2] = {make_uint4(so[0], so[1], so[2], so[3]), make_uint4(so[4], so[5], so[6], so[7])};
+            store_units<2>(p.d2 + (int64_t)grow * p.ldd2 + (col0 >> 1), us, (p.n - col0) >> 4, p.d2_v8);
+          }
+        }
+      }
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  // A pair leaves together: the peer may still signal this CTA's barriers until both are done.
+  if constexpr (CG == 2) ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    if constexpr (CG == 2) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+    else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+template <int BN, int EPI, bool B_MN, int CG>
+int launch(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
+  auto kern = gemm_kernel<BN, EPI, B_MN, CG>;
+  constexpr int smem = Cfg<BN, CG>::SMEM_BYTES;
+  static std::mutex mu;
+  static bool attr_done[64] = {};
+  static int max_units[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MGF_ERR_CUDA;
+  int units = sms / CG;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CG;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  {
+    std::lock_guard<std::mutex> g(mu);
+    if (!attr_done[dev]) {
+      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) {
+        record_error("cudaFuncSetAttribute", e);
+        return MGF_ERR_CUDA;
+      }
+      max_units[dev] = 1 << 30;
+      if (CG == 2) {  // never more persistent pairs than can be resident at once
+        int n = 0;
+        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) max_units[dev] = n;
+        cudaGetLastError();
+      }
+      attr_done[dev] = true;
+    }
+  }
+  if (units > max_units[dev]) units = max_units[dev];
+  if (tiles < units) units = static_cast<int>(tiles);
+  cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
+  cudaGetLastError();
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tA, tB, p);
+  if (e == cudaSuccess && debug_sync()) {
+    e = cudaStreamSynchronize(st);
+    fprintf(stderr, "[mgf] block-scaled BN=%d CG=%d epi=%d b_mn=%d units=%d E=%d rows=%lld n=%d k=%d -> %s\n", BN, CG,
+            EPI, int(B_MN), units, p.E, (long long)p.total_rows, p.n, p.k, cudaGetErrorString(e));
+  }
+  if (e != cudaSuccess) {
+    record_error("kernel launch", e);
+    return MGF_ERR_CUDA;
+  }
+  return MGF_OK;
+}
+
+template <int BN, int CG>
+int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+             cudaStream_t st) {
+  switch (epi) {
+    case MGF_EPI_BIAS:
+      return b_mn ? launch<BN, MGF_EPI_BIAS, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_BIAS, false, CG>(tA, tB, p, tiles, sms, st);
+    case MGF_EPI_SWIGLU:
+      return b_mn ? launch<BN, MGF_EPI_SWIGLU, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_SWIGLU, false, CG>(tA, tB, p, tiles, sms, st);
+    default:
+      return b_mn ? launch<BN, MGF_EPI_SWIGLU_BWD, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_SWIGLU_BWD, false, CG>(tA, tB, p, tiles, sms, st);
+  }
+}
+
+bool aligned(const void* ptr, unsigned n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1u)) == 0; }
+
+}  // namespace block_gemm
+}  // namespace mgf
+
+extern "C" size_t mgf_block_gemm_desc_size(void) { return sizeof(mgf_block_gemm_desc); }
+
+extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stream) {
+  using namespace mgf;
+  using namespace mgf::block_gemm;
+  if (desc == nullptr) return MGF_ERR_INVALID_ARGUMENT;
+  const mgf_block_gemm_desc& g = *desc;
+  if (g.num_groups < 1 || g.num_groups > kMaxGroups) return MGF_ERR_TOO_MANY_GROUPS;
+  if (g.epilogue < MGF_EPI_BIAS || g.epilogue > MGF_EPI_SWIGLU_BWD) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.total_rows < 0 || g.total_rows > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.n <= 0 || g.k <= 0 || g.n > INT32_MAX / 2 || g.k > INT32_MAX / 2 || g.n % 8 != 0) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.epilogue == MGF_EPI_SWIGLU && (g.n % 16 != 0 || g.d2 == nullptr || g.bias == nullptr))
+    return MGF_ERR_INVALID_ARGUMENT;
+  if (g.epilogue == MGF_EPI_SWIGLU_BWD && g.aux == nullptr) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.total_rows == 0) return MGF_OK;
+  if (g.a == nullptr || g.b == nullptr || g.offs == nullptr || g.scale_a == nullptr || g.scale_b == nullptr ||
+      g.d == nullptr)
+    return MGF_ERR_INVALID_ARGUMENT;
+  auto out_ok = [](const void* ptr, int64_t ld) { return aligned(ptr, 16) && ld > 0 && ld % 8 == 0; };
+  if (!aligned(g.a, 16) || !aligned(g.b, 16) || g.lda <= 0 || g.lda % 16 != 0 || g.ldb <= 0 || g.ldb % 16 != 0 ||
+      g.ldb_batch < 0 || g.ldb_batch % 16 != 0 || (g.num_groups > 1 && g.ldb_batch == 0) || !out_ok(g.d, g.ldd))
+    return MGF_ERR_ALIGNMENT;
+  if (g.epilogue == MGF_EPI_SWIGLU && !out_ok(g.d2, g.ldd2)) return MGF_ERR_ALIGNMENT;
+  if (g.epilogue == MGF_EPI_SWIGLU_BWD && !out_ok(g.aux, g.ld_aux)) return MGF_ERR_ALIGNMENT;
+  if (g.bias != nullptr && (!aligned(g.bias, 16) || g.bias_stride % 8 != 0)) return MGF_ERR_ALIGNMENT;
+
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return MGF_ERR_CUDA;
+  clear_error();
+  if (!bind_device(dev)) return MGF_ERR_CUDA;
+  const DeviceInfo di = device_info(dev);
+  if (di.major != 10) return MGF_ERR_NO_DEVICE_SUPPORT;
+
+  auto v8 = [](const void* ptr, int64_t ld) { return ptr != nullptr && aligned(ptr, 32) && ld % 16 == 0 ? 1 : 0; };
+  Params p{};
+  p.E = g.num_groups;
+  p.n = static_cast<int>(g.n);
+  p.k = static_cast<int>(g.k);
+  p.total_rows = g.total_rows;
+  p.offs = g.offs;
+  p.scale_a = g.scale_a;
+  p.lds_a = g.scale_a_stride;
+  p.scale_b = g.scale_b;
+  p.sb_e = g.scale_b_stride_e;
+  p.sb_k = g.scale_b_stride_k;
+  p.sb_n = g.scale_b_stride_n;
+  p.bias = g.epilogue == MGF_EPI_SWIGLU_BWD ? nullptr : static_cast<const __nv_bfloat16*>(g.bias);
+  p.bias_stride = g.bias_stride;
+  p.d = static_cast<__nv_bfloat16*>(g.d);
+  p.ldd = g.ldd;
+  p.d2 = static_cast<__nv_bfloat16*>(g.d2);
+  p.ldd2 = g.ldd2;
+  p.aux = static_cast<const __nv_bfloat16*>(g.aux);
+  p.ld_aux = g.ld_aux;
+  p.alpha = g.swiglu_alpha;
+  p.limit = g.swiglu_limit;
+  p.d_v8 = v8(g.d, g.ldd);
+  p.d2_v8 = v8(g.d2, g.ldd2);
+  p.aux_v8 = v8(g.aux, g.ld_aux);
+  p.status = status_word_address();
+  if (p.status == nullptr) return MGF_ERR_CUDA;
+  {
+    const char* env = getenv("MGF_TEST_STALL_PRODUCER");  // see moe_gemm_sm100.cu
+    p.stall_test = (env != nullptr && env[0] == '1') ? 1 : 0;
+  }
+
+  // Pairs (256-row tiles, half the B bytes per SM) for groups of 512 rows and more on average, as in
+  // moe_gemm_sm100.cu; MGF_CTA_GROUP=1|2 forces.  128-column tiles only where one covers n.
+  const bool b_mn = g.b_mn_major != 0;
+  int cg = g.total_rows / g.num_groups >= 512 ? 2 : 1;
+  if (const char* env = getenv("MGF_CTA_GROUP"); env != nullptr && (env[0] == '1' || env[0] == '2')) cg = env[0] - '0';
+  int bn = g.n <= 128 ? 128 : 256;
+  if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
+  if (bn == 128) cg = 1;
+  p.n_tiles = static_cast<int>((g.n + bn - 1) / bn);
+
+  CUtensorMap tA, tB;
+  const uint64_t dA[2] = {static_cast<uint64_t>(g.k), static_cast<uint64_t>(g.total_rows)};
+  const uint64_t sA[1] = {static_cast<uint64_t>(g.lda)};
+  const uint32_t bA[2] = {BK, BM};
+  const uint64_t batch = g.num_groups > 1 ? static_cast<uint64_t>(g.ldb_batch) : 16;
+  const uint64_t sB[2] = {static_cast<uint64_t>(g.ldb), batch};
+  const uint64_t dB_mn[3] = {static_cast<uint64_t>(g.n), static_cast<uint64_t>(g.k), static_cast<uint64_t>(g.num_groups)};
+  const uint64_t dB_k[3] = {static_cast<uint64_t>(g.k), static_cast<uint64_t>(g.n), static_cast<uint64_t>(g.num_groups)};
+  const uint32_t bB_mn[3] = {128, BK, 1};
+  const uint32_t bB_k[3] = {BK, static_cast<uint32_t>(bn / cg), 1};
+  const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  if (!encode_bf16(&tA, g.a, 2, dA, sA, bA, CU_TENSOR_MAP_SWIZZLE_128B, u8) ||
+      !encode_bf16(&tB, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bB_k, CU_TENSOR_MAP_SWIZZLE_128B, u8))
+    return MGF_ERR_CUDA;
+
+  const int64_t tiles = (g.total_rows / (BM * cg) + g.num_groups) * static_cast<int64_t>(p.n_tiles);  // upper bound
+  if (tiles > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
+  int sms = di.sms - (g.sm_carveout > 0 ? g.sm_carveout : 0);
+  if (sms < cg) sms = cg;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
+  if (cg == 2) return dispatch<256, 2>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
+  return dispatch<256, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
+}

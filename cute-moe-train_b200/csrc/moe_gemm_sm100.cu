@@ -40,6 +40,8 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "epilogue.cuh"
+#include "host.h"
 #include "moe_gemm.h"
 #include "ptx.cuh"
 
@@ -161,48 +163,6 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
 }
 
 
-#ifndef MGF_AUX_NOALLOC
-#define MGF_AUX_NOALLOC 1
-#endif
-// One chunk of aux words (32 packed (gate, up) pairs = 128 bytes of one row) as four 32-byte loads;
-// words past n read as zero.  Each sector is requested once, so nothing relies on L1 reuse.
-// v8 = false (aux rows only 16-byte aligned): eight 16-byte loads.
-__device__ __forceinline__ void load_aux_chunk(const __nv_bfloat16* row, int col0, int n, bool valid, bool v8,
-                                               uint4 (&aw)[8]) {
-  const uint4* ap = reinterpret_cast<const uint4*>(row + 2 * col0);
-  if (!v8) {
-#pragma unroll
-    for (int g = 0; g < 8; ++g) aw[g] = (valid && col0 + 4 * g < n) ? __ldg(ap + g) : make_uint4(0, 0, 0, 0);
-    return;
-  }
-#pragma unroll
-  for (int g = 0; g < 8; g += 2) {
-    if (valid && col0 + 4 * g < n) {
-      if (MGF_AUX_NOALLOC) ptx::ld_nc_v8_noalloc(ap + g, aw[g], aw[g + 1]);
-      else ptx::ld_nc_v8(ap + g, aw[g], aw[g + 1]);
-    } else {
-      aw[g] = make_uint4(0, 0, 0, 0);
-      aw[g + 1] = make_uint4(0, 0, 0, 0);
-    }
-  }
-}
-
-// Store the first `nvalid` of NU 16-byte units of one output row; pairs of units go out as one
-// 32-byte store when v8 (the row and its 32-byte pairs aligned).
-template <int NU>
-__device__ __forceinline__ void store_units(void* dst, const uint4 (&u)[NU], int nvalid, bool v8) {
-  uint4* d = reinterpret_cast<uint4*>(dst);
-#pragma unroll
-  for (int g = 0; g < NU; g += 2) {
-    if (v8 && g + 1 < nvalid) {
-      ptx::st_v8(d + g, u[g], u[g + 1]);
-    } else {
-      if (g < nvalid) d[g] = u[g];
-      if (g + 1 < nvalid) d[g + 1] = u[g + 1];
-    }
-  }
-}
-
 template <int TM, bool RAGGED_K>
 __device__ __forceinline__ void decode_tile(int t, const Params& p, const SchedSmem& s, TileInfo& ti) {
   int lo = 0, hi = p.E;
@@ -273,44 +233,6 @@ __device__ void build_schedule(const Params& p, const SchedSmem& s, int lane) {
   }
   if (lane == 0) s.prefix[0] = 0;
   if (__any_sync(0xffffffffu, bad) && lane == 0) atomicOr(&g_status, MGF_DEV_BAD_OFFS);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-
-// sigma(z) = 0.5 * tanh(z / 2) + 0.5, the form the reference's SwiGLU visitors use
-// (csrc/grouped_mm_swiglu_visitor.cuh:309-334, csrc/grouped_mm_swiglu_bwd_visitor.cuh:35-68), on the
-// hardware tanh approximation (one MUFU operation; max relative error about 2^-11, below bf16's 2^-8).
-__device__ __forceinline__ float tanh_approx(float x) {
-  float y;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float sigmoidf_fast(float z) { return fmaf(0.5f, tanh_approx(0.5f * z), 0.5f); }
-
-// SwiGLU forward on one (gate, up) pair of bf16-rounded values.
-__device__ __forceinline__ float swiglu_fwd(float g, float u, float alpha, float limit) {
-  const float gc = fminf(g, limit);
-  const float uc = fmaxf(fminf(u, limit), -limit);
-  return gc * sigmoidf_fast(alpha * gc) * (uc + 1.0f);
-}
-
-// SwiGLU backward for one packed (gate, up) word of aux; returns packed (d_gate, d_up).
-__device__ __forceinline__ uint32_t swiglu_bwd_word(float gs, uint32_t aux_word, float alpha, float limit) {
-  const float g = bf16_lo(aux_word);
-  const float u = bf16_hi(aux_word);
-  const float gc = fminf(g, limit);
-  const float uc = fmaxf(fminf(u, limit), -limit);
-  const float sig = sigmoidf_fast(alpha * gc);
-  float d_gate = gs * (uc + 1.0f) * sig * (1.0f + alpha * gc * (1.0f - sig));
-  float d_up = gs * gc * sig;
-  d_gate = (g <= limit) ? d_gate : 0.0f;
-  d_up = (u >= -limit && u <= limit) ? d_up : 0.0f;
-  return pack_bf16x2(d_gate, d_up);
 }
 
 // Zero the K rows valid_k..end_k-1 (past the group end, up to the last row the MMAs read) in this
@@ -1077,9 +999,8 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
-static bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
-                        const uint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B,
-                        CUtensorMapDataType dtype = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16) {
+bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dims, const uint64_t* strides_bytes,
+                 const uint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapDataType dtype) {
   EncodeTiledFn fn = get_encode_fn();
   if (fn == nullptr) return false;
   if (rank < 1 || rank > 4) return false;
@@ -1102,12 +1023,7 @@ static bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64
   return true;
 }
 
-struct DeviceInfo {
-  int sms = 0;
-  int major = 0;
-};
-
-static DeviceInfo device_info(int dev) {
+DeviceInfo device_info(int dev) {
   static DeviceInfo cache[64];
   static std::mutex mu;
   std::lock_guard<std::mutex> g(mu);
@@ -1119,11 +1035,25 @@ static DeviceInfo device_info(int dev) {
   return cache[dev];
 }
 
-static void record_error(const char* what, cudaError_t e) {
+void clear_error() { g_last_error[0] = 0; }
+
+// Tensor maps are encoded through the driver API, which needs a current context on this host
+// thread.  Threads that only made runtime calls so far (autograd's backward workers) may have
+// none; cudaSetDevice binds the device's primary context.
+bool bind_device(int dev) {
+  static thread_local int bound_dev = -1;
+  if (bound_dev != dev) {
+    if (cudaSetDevice(dev) != cudaSuccess) return false;
+    bound_dev = dev;
+  }
+  return true;
+}
+
+void record_error(const char* what, cudaError_t e) {
   snprintf(g_last_error, sizeof(g_last_error), "%s: %s", what, cudaGetErrorString(e));
 }
 
-static bool debug_sync() {
+bool debug_sync() {
   static int v = -1;
   if (v < 0) {
     const char* e = getenv("MGF_DEBUG_SYNC");
@@ -1352,15 +1282,8 @@ extern "C" int mgf_grouped_gemm_launch(const mgf_gemm_desc* desc, void* stream) 
 
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return MGF_ERR_CUDA;
-  g_last_error[0] = 0;
-  // Tensor maps are encoded through the driver API, which needs a current context on this host
-  // thread.  Threads that only made runtime calls so far (autograd's backward workers) may have
-  // none; cudaSetDevice binds the device's primary context.
-  static thread_local int bound_dev = -1;
-  if (bound_dev != dev) {
-    if (cudaSetDevice(dev) != cudaSuccess) return MGF_ERR_CUDA;
-    bound_dev = dev;
-  }
+  clear_error();
+  if (!bind_device(dev)) return MGF_ERR_CUDA;
   const DeviceInfo di = device_info(dev);
   if (di.major != 10) return MGF_ERR_NO_DEVICE_SUPPORT;
 

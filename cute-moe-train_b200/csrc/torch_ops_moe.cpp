@@ -294,6 +294,124 @@ std::tuple<Tensor, Tensor> quantize_weights_block_cuda(const Tensor& w) {
   return {q.transpose(1, 2), scale.transpose(1, 2)};
 }
 
+// ---------------------------------------------------------------- grouped product of block-scaled operands
+// Stride of dimension i; a dimension of one element may carry any.
+int64_t stride_of(const Tensor& t, int i, int64_t otherwise) { return t.size(i) > 1 ? t.stride(i) : otherwise; }
+
+struct BlockArgs {
+  mgf_block_gemm_desc g{};
+  int64_t rows, n;
+};
+
+BlockArgs block_args(const Tensor& a, const Tensor& b, const Tensor& offs, const Tensor& scale_a, const Tensor& scale_b,
+                     const std::optional<Tensor>& bias, const char* what) {
+  TORCH_CHECK(a.is_cuda() && b.is_cuda(), what, ": inputs must be CUDA tensors");
+  TORCH_CHECK(a.dim() == 2 && b.dim() == 3, what, ": mat_a must be 2D and mat_b 3D");
+  TORCH_CHECK(a.scalar_type() == at::kFloat8_e4m3fn && b.scalar_type() == at::kFloat8_e4m3fn, what,
+              ": mat_a and mat_b must be float8_e4m3fn");
+  const int64_t M = a.size(0), K = a.size(1), E = b.size(0), N = b.size(2);
+  TORCH_CHECK(b.size(1) == K, what, ": contraction dimension of mat_a and mat_b must match");
+  TORCH_CHECK(K >= 1 && N >= 1 && N % 8 == 0, what, ": N must be a positive multiple of 8 and K positive, got N=", N,
+              ", K=", K);
+  TORCH_CHECK(offs.scalar_type() == at::kInt && offs.dim() == 1 && offs.is_contiguous() && offs.size(0) == E, what,
+              ": offs must be a contiguous int32 [E] tensor");
+  TORCH_CHECK(E >= 1 && E <= 1024, what, ": group count must be in [1, 1024], got ", E);
+  for (const Tensor* t : {&b, &offs, &scale_a, &scale_b})
+    TORCH_CHECK(t->device() == a.device(), what, ": all tensors must be on the same device");
+  TORCH_CHECK((K == 1 || a.stride(1) == 1) && (M <= 1 || a.stride(0) >= K), what, ": mat_a must be row-major");
+  const bool mn = N == 1 || b.stride(2) == 1;
+  TORCH_CHECK(mn || K == 1 || b.stride(1) == 1, what, ": mat_b must have unit stride along N or K");
+  TORCH_CHECK(scale_a.scalar_type() == at::kFloat && scale_a.dim() == 2 && scale_a.size(0) == M &&
+                  scale_a.size(1) == blocks_of(K) && (scale_a.size(1) == 1 || scale_a.stride(1) == 1),
+              what, ": scale_a must be float32 [M, ceil(K / 128)] with unit stride along the blocks");
+  TORCH_CHECK(scale_b.scalar_type() == at::kFloat && scale_b.dim() == 3 && scale_b.size(0) == E &&
+                  scale_b.size(1) == blocks_of(K) && scale_b.size(2) == blocks_of(N),
+              what, ": scale_b must be float32 [E, ceil(K / 128), ceil(N / 128)]");
+  if (bias.has_value())
+    TORCH_CHECK(bias->device() == a.device() && bias->scalar_type() == at::kBFloat16 && bias->dim() == 2 &&
+                    bias->size(0) == E && bias->size(1) == N && bias->is_contiguous(),
+                what, ": bias must be a contiguous BFloat16 [E, N] tensor");
+  BlockArgs r;
+  mgf_block_gemm_desc& g = r.g;
+  r.rows = M;
+  r.n = N;
+  g.num_groups = static_cast<int32_t>(E);
+  g.total_rows = M;
+  g.n = N;
+  g.k = K;
+  g.a = a.data_ptr();
+  g.lda = stride_of(a, 0, round_up(K, 16));
+  g.b = b.data_ptr();
+  g.b_mn_major = mn ? 1 : 0;
+  g.ldb = mn ? stride_of(b, 1, round_up(N, 16)) : stride_of(b, 2, round_up(K, 16));
+  g.ldb_batch = stride_of(b, 0, 16);
+  g.offs = offs.data_ptr<int32_t>();
+  g.scale_a = scale_a.data_ptr<float>();
+  g.scale_a_stride = scale_a.stride(0);
+  g.scale_b = scale_b.data_ptr<float>();
+  g.scale_b_stride_e = scale_b.stride(0);
+  g.scale_b_stride_k = scale_b.stride(1);
+  g.scale_b_stride_n = scale_b.stride(2);
+  if (bias.has_value()) {
+    g.bias = bias->data_ptr();
+    g.bias_stride = N;
+  }
+  const auto carve = at::globalContext()._SMCarveout_EXPERIMENTAL();
+  g.sm_carveout = carve.has_value() ? static_cast<int32_t>(*carve) : 0;
+  return r;
+}
+
+Tensor mm_fp8_block_cuda(const Tensor& a, const Tensor& b, const Tensor& offs, const Tensor& scale_a,
+                         const Tensor& scale_b, const std::optional<Tensor>& bias) {
+  BlockArgs r = block_args(a, b, offs, scale_a, scale_b, bias, "grouped_mm_fp8_block");
+  const c10::cuda::CUDAGuard guard(a.device());
+  Tensor out = padded_rows(r.rows, r.n, a.options().dtype(at::kBFloat16));
+  r.g.epilogue = MGF_EPI_BIAS;
+  r.g.d = out.data_ptr();
+  r.g.ldd = out.stride(0);
+  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_fp8_block");
+  return out;
+}
+
+std::tuple<Tensor, Tensor> mm_swiglu_fp8_block_cuda(const Tensor& a, const Tensor& b, const Tensor& offs,
+                                                    const Tensor& scale_a, const Tensor& scale_b, const Tensor& bias,
+                                                    double alpha, double limit) {
+  BlockArgs r = block_args(a, b, offs, scale_a, scale_b, bias, "grouped_mm_swiglu_fp8_block");
+  TORCH_CHECK(r.n % 16 == 0, "grouped_mm_swiglu_fp8_block: 2*I must be a multiple of 16, got ", r.n);
+  const c10::cuda::CUDAGuard guard(a.device());
+  Tensor s = padded_rows(r.rows, r.n / 2, a.options().dtype(at::kBFloat16));
+  Tensor aux = padded_rows(r.rows, r.n, a.options().dtype(at::kBFloat16));
+  r.g.epilogue = MGF_EPI_SWIGLU;
+  r.g.d = aux.data_ptr();
+  r.g.ldd = aux.stride(0);
+  r.g.d2 = s.data_ptr();
+  r.g.ldd2 = s.stride(0);
+  r.g.swiglu_alpha = static_cast<float>(alpha);
+  r.g.swiglu_limit = static_cast<float>(limit);
+  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_swiglu_fp8_block");
+  return {s, aux};
+}
+
+Tensor mm_swiglu_bwd_fp8_block_cuda(const Tensor& grad_output, const Tensor& down_w_t, const Tensor& offs,
+                                    const Tensor& aux, const Tensor& scale_a, const Tensor& scale_b, double alpha,
+                                    double limit) {
+  BlockArgs r = block_args(grad_output, down_w_t, offs, scale_a, scale_b, std::nullopt, "grouped_mm_swiglu_bwd_fp8_block");
+  TORCH_CHECK(aux.device() == grad_output.device() && aux.scalar_type() == at::kBFloat16 && aux.dim() == 2 &&
+                  aux.size(0) == r.rows && aux.size(1) == 2 * r.n && aux.stride(1) == 1,
+              "grouped_mm_swiglu_bwd_fp8_block: aux_biased_acc must be a row-major BFloat16 [M, 2*I] tensor");
+  const c10::cuda::CUDAGuard guard(grad_output.device());
+  Tensor out = padded_rows(r.rows, 2 * r.n, aux.options());
+  r.g.epilogue = MGF_EPI_SWIGLU_BWD;
+  r.g.d = out.data_ptr();
+  r.g.ldd = out.stride(0);
+  r.g.aux = aux.data_ptr();
+  r.g.ld_aux = stride_of(aux, 0, round_up(2 * r.n, 8));
+  r.g.swiglu_alpha = static_cast<float>(alpha);
+  r.g.swiglu_limit = static_cast<float>(limit);
+  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_swiglu_bwd_fp8_block");
+  return out;
+}
+
 // ---------------------------------------------------------------- autograd of the router and the permutation
 template <typename F>
 auto op(const char* name) {
@@ -486,6 +604,14 @@ TORCH_LIBRARY_FRAGMENT(grouped_mm, m) {
   m.def("fp8_quantize_rows_block(Tensor x) -> (Tensor, Tensor)");
   m.def("fp8_quantize_weights_block(Tensor w) -> (Tensor, Tensor)");
   m.def("moe_permute_fp8(Tensor x, Tensor expert_idx, int num_experts) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def(
+      "mm_fp8_block(Tensor mat_a, Tensor mat_b, Tensor offs, Tensor scale_a, Tensor scale_b, Tensor? bias) -> Tensor");
+  m.def(
+      "mm_swiglu_fp8_block(Tensor mat_a, Tensor mat_b, Tensor offs, Tensor scale_a, Tensor scale_b, Tensor bias,"
+      " float swiglu_alpha, float swiglu_limit) -> (Tensor, Tensor)");
+  m.def(
+      "mm_swiglu_bwd_fp8_block(Tensor grad_output, Tensor down_w_t, Tensor offs, Tensor aux_biased_acc, Tensor scale_a,"
+      " Tensor scale_b, float swiglu_alpha, float swiglu_limit) -> Tensor");
   m.def("moe_permute_rows_fp8(Tensor x, Tensor offs, Tensor row_of_copy) -> (Tensor, Tensor)");
 }
 
@@ -500,6 +626,9 @@ TORCH_LIBRARY_IMPL(grouped_mm, CUDA, m) {
   m.impl("fp8_quantize_rows_block", &quantize_rows_block_cuda);
   m.impl("fp8_quantize_weights_block", &quantize_weights_block_cuda);
   m.impl("moe_permute_fp8", &moe_permute_fp8_cuda);
+  m.impl("mm_fp8_block", &mm_fp8_block_cuda);
+  m.impl("mm_swiglu_fp8_block", &mm_swiglu_fp8_block_cuda);
+  m.impl("mm_swiglu_bwd_fp8_block", &mm_swiglu_bwd_fp8_block_cuda);
   m.impl("moe_permute_rows_fp8", &permute_rows_fp8_cuda);
 }
 

@@ -1,10 +1,16 @@
-"""e4m3 with a scale for each block of 128: quantisers.
+"""e4m3 with a scale for each block of 128: quantisers, grouped products and the FFN with autograd.
 
 The recipe of :mod:`fp8` gives a whole row or column one scale, so one outlier costs all of it its small
 values.  Here every 1 x 128 block of an activation row and every 128 x 128 block of a weight has its own.
 The scales are powers of two (the smallest s with amax / s <= 448), so quantising rounds only once, in the
 code; the grouped product takes any fp32 scales.  The weights' codes keep the weights' layout: one set is
 the forward's operand and, transposed, the input gradient's.
+
+``grouped_mm_fp8_block``, ``grouped_mm_swiglu_fp8_block`` and ``grouped_mm_swiglu_bwd_fp8_block`` are the
+ragged-M products with the bias, SwiGLU and SwiGLU-backward epilogues; every block's product is scaled and
+added in fp32.  ``grouped_mm_ffn_fp8_block`` chains them into the MoE FFN with autograd: both forward products
+and both input gradients in e4m3, the weight and bias gradients in bf16 (``grouped_mm::mm_wgrad_bias``) from the
+unquantised activations -- they contract over tokens, where the 1 x 128 blocks of either operand do not lie.
 """
 
 from __future__ import annotations
@@ -12,6 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext  # noqa: F401  (registers the operators)
+from .custom_op import _padded
 from .optimer import timed
 from .permute import _codes_fake
 
@@ -62,3 +69,56 @@ def dequantize_rows_block(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 def dequantize_weights_block(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
     s = scale.repeat_interleave(BLOCK, 1)[:, :q.shape[1]].repeat_interleave(BLOCK, 2)[:, :, :q.shape[2]]
     return q.float() * s
+
+
+def _out_fake(mat_a, cols):
+    return torch.empty_strided((mat_a.size(0), cols), (_padded(cols, torch.bfloat16), 1), dtype=torch.bfloat16,
+                               device=mat_a.device)
+
+
+@torch.library.register_fake("grouped_mm::mm_fp8_block")
+def _mm_fp8_block_fake(mat_a, mat_b, offs, scale_a, scale_b, bias):
+    return _out_fake(mat_a, mat_b.size(2))
+
+
+@torch.library.register_fake("grouped_mm::mm_swiglu_fp8_block")
+def _mm_swiglu_fp8_block_fake(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha, swiglu_limit):
+    return _out_fake(mat_a, mat_b.size(2) // 2), _out_fake(mat_a, mat_b.size(2))
+
+
+@torch.library.register_fake("grouped_mm::mm_swiglu_bwd_fp8_block")
+def _mm_swiglu_bwd_fp8_block_fake(grad_output, down_w_t, offs, aux_biased_acc, scale_a, scale_b, swiglu_alpha,
+                                  swiglu_limit):
+    return _out_fake(grad_output, 2 * down_w_t.size(2))
+
+
+def grouped_mm_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.Tensor, scale_a: torch.Tensor,
+                         scale_b: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
+    """Ragged-M grouped product of block-scaled e4m3 operands (+ per-expert bf16 bias) -> bf16 [total_M, N].
+
+    mat_a e4m3 [total_M, K] row-major and mat_b e4m3 [E, K, N] with unit stride along N or K (rows 16 bytes
+    apart), scale_a fp32 [total_M, ceil(K / 128)], scale_b fp32 [E, ceil(K / 128), ceil(N / 128)] (any strides),
+    offs int32 [E] cumulative row ends, N a multiple of 8.  Rows behind offs[-1] are not written.
+    """
+    with timed("fp8_block_mm"):
+        return torch.ops.grouped_mm.mm_fp8_block(mat_a, mat_b, offs, scale_a, scale_b, bias)
+
+
+def grouped_mm_swiglu_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.Tensor, scale_a: torch.Tensor,
+                                scale_b: torch.Tensor, bias: torch.Tensor, swiglu_alpha: float = 1.702,
+                                swiglu_limit: float = 7.0) -> tuple[torch.Tensor, torch.Tensor]:
+    """The product + bias + clamped SwiGLU -> (swiglu_out [total_M, I], aux_biased_acc [total_M, 2I]), the
+    activation computed from the stored (bf16) aux; mat_b's columns interleave gate and up."""
+    with timed("fp8_block_up_swiglu_fwd"):
+        return torch.ops.grouped_mm.mm_swiglu_fp8_block(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha,
+                                                        swiglu_limit)
+
+
+def grouped_mm_swiglu_bwd_fp8_block(grad_output: torch.Tensor, down_w_t: torch.Tensor, offs: torch.Tensor,
+                                    aux_biased_acc: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
+                                    swiglu_alpha: float = 1.702, swiglu_limit: float = 7.0) -> torch.Tensor:
+    """SwiGLU backward of the product grad_output @ down_w_t against aux -> grad_aux bf16 [total_M, 2I]
+    (interleaved like aux)."""
+    with timed("fp8_block_down_dgrad_swiglu_bwd"):
+        return torch.ops.grouped_mm.mm_swiglu_bwd_fp8_block(grad_output, down_w_t, offs, aux_biased_acc, scale_a,
+                                                            scale_b, swiglu_alpha, swiglu_limit)

@@ -309,6 +309,47 @@ int mgf_fp8_block_quantize_weights(const void* w, int64_t E, int64_t R, int64_t 
                                    int64_t q_e, int64_t q_r, float* scale, int64_t ss_e, int64_t ss_r, int64_t ss_c,
                                    void* stream);
 
+/* Grouped GEMM of e4m3 operands with a scale per block of 128 (ragged M; epilogues BIAS, SWIGLU and
+ * SWIGLU_BWD, the fields that mgf_gemm_desc has too as there):
+ *   acc[r, c] = sum_b scale_a[r, b] * scale_b[e, b, c / 128] * sum_{k in block b} a[r, k] * b[e, k, c]
+ * with fp32 accumulation of every block and of their sum.  Any fp32 scales, not only powers of two.
+ *   a       e4m3 [total_rows, k], unit stride along k, row stride lda (bytes, a multiple of 16)
+ *   b       e4m3 [E, k, n]: b_mn_major 1: unit stride along n, ldb between k rows; 0: unit stride along k, ldb
+ *           between columns (bytes, multiples of 16; ldb_batch between groups likewise)
+ *   scale_a fp32 [total_rows, ceil(k / 128)], unit stride along the blocks, row stride scale_a_stride
+ *   scale_b fp32 [E, ceil(k / 128), ceil(n / 128)] with any strides
+ *   n a multiple of 8 (SWIGLU: 16), k any; outputs as for mgf_gemm_desc (16-byte rules).  Rows behind
+ *   offs[E-1] are not written. */
+typedef struct mgf_block_gemm_desc {
+  int32_t epilogue;
+  int32_t num_groups;
+  int64_t total_rows, n, k;
+  const void* a;
+  int64_t lda;
+  const void* b;
+  int64_t ldb, ldb_batch;
+  int32_t b_mn_major;
+  int32_t sm_carveout;
+  const int32_t* offs;
+  const float* scale_a;
+  int64_t scale_a_stride;
+  const float* scale_b;
+  int64_t scale_b_stride_e, scale_b_stride_k, scale_b_stride_n;
+  const void* bias;
+  int64_t bias_stride;
+  void* d;
+  int64_t ldd;
+  void* d2;
+  int64_t ldd2;
+  const void* aux;
+  int64_t ld_aux;
+  float swiglu_alpha;
+  float swiglu_limit;
+} mgf_block_gemm_desc;
+
+int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stream);
+size_t mgf_block_gemm_desc_size(void);
+
 /* Map a peer process's device allocation (its 64-byte cudaIpcMemHandle_t) into the context of
  * the calling thread's current device, peer access enabled, for mgf_push_rows destinations
  * (no counterpart in the reference).  mgf_ipc_close unmaps it. */

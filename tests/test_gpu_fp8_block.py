@@ -1,4 +1,14 @@
-"""e4m3 with a scale per block of 128: quantisers against their definition (bit for bit)."""
+"""e4m3 with a scale per block of 128: quantisers against their definition (bit for bit), the grouped
+products against the same sums in 64 bits.
+
+Tolerances of the products count roundings (u = 2^-24).  A block of 128 products of e4m3 numbers is summed
+by the tensor core: the products are exact (8 significant bits), the sum of 128 is allowed 128 roundings that
+may truncate instead of round (2 u each); the scale factor sa * sb rounds once, the promotion (one fused
+multiply-add per block) once per block.  So |acc - exact| <= (256 + 1 + blocks) u * S with S the sum of the
+magnitudes of all products.  bf16 output: 2^-8 of the value.  SwiGLU and its backward are computed from
+bf16 (exactly known) or fp32 inputs in fp32: a few u times their condition, below 64 u of the terms'
+magnitudes, times the output rounding.
+"""
 
 from __future__ import annotations
 
@@ -38,7 +48,7 @@ def _rows_ref(x):
     full[:, :k] = x.double()
     b = full.view(m, nb, 128)
     s = _scale_ref(torch.where(torch.isfinite(b), b, 0.0).abs().amax(2))
-    return _code_ref(b, s[:, :, None]).reshape(m, -1)[:, :k], s
+    return _code_ref(b, s[:, :, None]).reshape(m, nb * 128)[:, :k], s
 
 
 def _weights_ref(w):
@@ -161,3 +171,198 @@ def test_quantiser_refusals():
         fp8_block.quantize_weights_block(torch.zeros(2, 8, 8, 2, device="cuda", dtype=torch.bfloat16)[..., 0])
     with pytest.raises(RuntimeError, match="bf16"):
         fp8_block.quantize_weights_block(torch.zeros(8, 8, device="cuda", dtype=torch.bfloat16))
+
+
+# ------------------------------------------------------------------------------------------------ grouped products
+U = 2.0 ** -24
+ALPHA, LIMIT = 1.702, 7.0
+
+
+def _case(E, K, N, counts, layout, seed, extra_rows=0):
+    """Operands with arbitrary fp32 scales (not powers of two); groups of `counts` rows and rows behind them."""
+    g = _gen(seed)
+    M = sum(counts) + extra_rows
+
+    def codes(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").mul_(20).to(torch.float8_e4m3fn)
+
+    def pitched(t):
+        p = torch.zeros(*t.shape[:-1], (t.shape[-1] + 15) // 16 * 16 + 16, dtype=t.dtype, device="cuda")
+        p = p[..., :t.shape[-1]]
+        p.copy_(t)
+        return p
+
+    kb, nb = -(-K // 128), -(-N // 128)
+    a = pitched(codes(M, K))
+    b = pitched(codes(E, K, N)) if layout == "kn" else pitched(codes(E, N, K)).transpose(1, 2)
+    sa = torch.empty(M, (kb + 3) // 4 * 4, device="cuda")[:, :kb]
+    sa.copy_(0.01 + torch.rand(M, kb, generator=g, device="cuda"))
+    sb = 0.01 + torch.rand(E, kb, nb, generator=g, device="cuda")
+    if layout == "nk":
+        sb = sb.transpose(1, 2).contiguous().transpose(1, 2)
+    offs = torch.tensor(counts, device="cuda").cumsum(0).int()
+    bias = (100 * torch.randn(E, N, generator=g, device="cuda")).to(torch.bfloat16)
+    return a, b, offs, sa, sb, bias
+
+
+def _exact(a, b, offs, sa, sb):
+    """(sum, sum of magnitudes) of every output, in 64 bits; rows behind the last group stay zero."""
+    K, N = b.shape[1:]
+    out = torch.zeros(a.shape[0], N, dtype=torch.float64, device="cuda")
+    mag = torch.zeros_like(out)
+    ad = a.double() * sa.double().repeat_interleave(128, 1)[:, :K]
+    lo = 0
+    for e, hi in enumerate(offs.tolist()):
+        s = sb[e].double().repeat_interleave(128, 0)[:K].repeat_interleave(128, 1)[:, :N]
+        bd = b[e].double() * s
+        out[lo:hi] = ad[lo:hi] @ bd
+        mag[lo:hi] = ad[lo:hi].abs() @ bd.abs()
+        lo = hi
+    return out, mag
+
+
+def _within(name, got, ref, tol):
+    over = (got.double() - ref).abs() - tol
+    worst = float(over.max()) if over.numel() else 0.0
+    assert not over.isnan().any() and worst <= 0.0, f"{name}: {int((over > 0).sum())} of {over.numel()} off by up to {worst:.3e}"
+
+
+def _row_of(offs, M):
+    """Group of every row (the last one's for rows behind it)."""
+    return torch.bucketize(torch.arange(M, device="cuda"), offs.long(), right=True).clamp(max=offs.numel() - 1)
+
+
+SHAPES = [
+    (1, 1, 16, [1]),
+    (1, 128, 128, [128]),
+    (4, 256, 192, [70, 0, 131, 5]),
+    (3, 320, 272, [600, 513, 700]),
+    (2, 2880, 528, [1029, 640]),
+    (5, 100, 48, [0, 1, 127, 129, 0]),
+    (2, 1000, 1040, [3, 260]),
+    (40, 136, 144, [1] * 40),
+]
+
+
+@pytest.mark.parametrize("form", ["auto", "single", "pair", "narrow"])
+@pytest.mark.parametrize("layout", ["kn", "nk"])
+@pytest.mark.parametrize("E,K,N,counts", SHAPES)
+def test_products_against_64_bits(E, K, N, counts, layout, form, monkeypatch):
+    import cutlass_op.bf16_grouped_mm as m
+    from cutlass_op.bf16_grouped_mm import fp8_block
+
+    if form in ("single", "pair"):
+        monkeypatch.setenv("MGF_CTA_GROUP", "1" if form == "single" else "2")
+    if form == "narrow":
+        monkeypatch.setenv("MGF_BN", "128")
+    a, b, offs, sa, sb, bias = _case(E, K, N, counts, layout, E * 7 + K, extra_rows=3)
+    rows = int(offs[-1])
+    acc, mag = _exact(a, b, offs, sa, sb)
+    tol = (257 + sa.shape[1]) * U * mag
+    out = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb)
+    _within("no bias", out[:rows], acc[:rows], (tol + 2.0 ** -8 * acc.abs())[:rows])
+    biased = acc + bias.double()[_row_of(offs, acc.shape[0])]
+    tol = tol + U * biased.abs()
+    out = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias)
+    _within("bias", out[:rows], biased[:rows], (tol + 2.0 ** -8 * biased.abs())[:rows])
+    # SwiGLU in a range where it is not all clamped
+    sa2 = sa * 2.0 ** -10
+    sa2 = torch.empty_strided(sa.shape, sa.stride(), device="cuda").copy_(sa2)
+    bias2 = (bias.float() / 64).to(torch.bfloat16)
+    acc2, mag2 = acc * 2.0 ** -10, mag * 2.0 ** -10
+    biased = acc2 + bias2.double()[_row_of(offs, acc.shape[0])]
+    s, aux = fp8_block.grouped_mm_swiglu_fp8_block(a, b, offs, sa2, sb, bias2, ALPHA, LIMIT)
+    _within("aux", aux[:rows], biased[:rows],
+            ((257 + sa.shape[1]) * U * mag2 + U * biased.abs() + 2.0 ** -8 * biased.abs())[:rows])
+    gate, up = aux.double()[:, 0::2].clamp(max=LIMIT), aux.double()[:, 1::2].clamp(-LIMIT, LIMIT)
+    ref = gate * torch.sigmoid(ALPHA * gate) * (up + 1)
+    # exp of an argument of up to |alpha gate| with a rounding of its own: |z| u; u + 1 loses |up| u absolutely
+    cond = (gate * torch.sigmoid(ALPHA * gate)).abs() * ((up + 1).abs() * (8 + 4 * (ALPHA * gate).abs()) + 2 * up.abs())
+    _within("swiglu", s[:rows], ref[:rows], (8 * U * cond + 2.0 ** -8 * ref.abs() + 1e-37)[:rows])
+    # SwiGLU backward against an aux with clamped and unclamped values
+    aux_in = (4 * torch.randn(a.shape[0], 2 * N, generator=_gen(9), device="cuda")).to(torch.bfloat16)
+    got = fp8_block.grouped_mm_swiglu_bwd_fp8_block(a, b, offs, aux_in, sa2, sb, ALPHA, LIMIT)
+    g0, u0 = aux_in.double()[:, 0::2], aux_in.double()[:, 1::2]
+    gc, uc = g0.clamp(max=LIMIT), u0.clamp(-LIMIT, LIMIT)
+    sig = torch.sigmoid(ALPHA * gc)
+    err = (257 + sa.shape[1]) * U * mag2
+    fg = (uc + 1) * sig * (1 + ALPHA * gc * (1 - sig)) * (g0 <= LIMIT)
+    fu = gc * sig * (u0.abs() <= LIMIT)
+    z = (ALPHA * gc).abs()
+    cg = sig * ((uc + 1).abs() * (1 + z) * (16 + 8 * z) + 2 * uc.abs() * (1 + z))
+    cu = gc.abs() * sig * (8 + 4 * z)
+    for name, f, c, part in (("d_gate", fg, cg, got[:, 0::2]), ("d_up", fu, cu, got[:, 1::2])):
+        ref = acc2 * f
+        _within(name, part[:rows], ref[:rows],
+                (err * (f.abs() + 8 * U * c) + 8 * U * c * acc2.abs() + 2.0 ** -8 * ref.abs() + 1e-37)[:rows])
+    m.check_device_status()
+
+
+def test_rows_behind_the_last_group_stay_as_they_were():
+    """The launcher writes rows of groups only: an output that the caller filled keeps the others."""
+    import ctypes
+
+    from cutlass_op.bf16_grouped_mm import _ext, fp8_block
+
+    a, b, offs, sa, sb, bias = _case(3, 256, 256, [5, 0, 130], "kn", 1, extra_rows=200)
+    want = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias)
+    out = torch.full((a.shape[0], 256), 7.0, dtype=torch.bfloat16, device="cuda")
+
+    class Desc(ctypes.Structure):  # include/moe_gemm.h: mgf_block_gemm_desc
+        i32, i64, ptr, f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
+        _fields_ = [("epilogue", i32), ("num_groups", i32), ("total_rows", i64), ("n", i64), ("k", i64), ("a", ptr),
+                    ("lda", i64), ("b", ptr), ("ldb", i64), ("ldb_batch", i64), ("b_mn_major", i32),
+                    ("sm_carveout", i32), ("offs", ptr), ("scale_a", ptr), ("scale_a_stride", i64), ("scale_b", ptr),
+                    ("scale_b_stride_e", i64), ("scale_b_stride_k", i64), ("scale_b_stride_n", i64), ("bias", ptr),
+                    ("bias_stride", i64), ("d", ptr), ("ldd", i64), ("d2", ptr), ("ldd2", i64), ("aux", ptr),
+                    ("ld_aux", i64), ("swiglu_alpha", f32), ("swiglu_limit", f32)]
+
+    _ext.lib.mgf_block_gemm_desc_size.restype = ctypes.c_size_t
+    assert ctypes.sizeof(Desc) == _ext.lib.mgf_block_gemm_desc_size()
+    d = Desc(0, 3, a.shape[0], 256, 256, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(1), b.stride(0), 1, 0,
+             offs.data_ptr(), sa.data_ptr(), sa.stride(0), sb.data_ptr(), *sb.stride(), bias.data_ptr(), 256,
+             out.data_ptr(), 256, None, 0, None, 0, ALPHA, LIMIT)
+    _ext.lib.mgf_block_gemm_launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
+    assert _ext.lib.mgf_block_gemm_launch(ctypes.byref(d), torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out[:135], want[:135]) and (out[135:] == 7.0).all()
+
+
+def test_malformed_offs_are_clamped_and_reported():
+    from cutlass_op.bf16_grouped_mm import fp8_block
+    from cutlass_op.bf16_grouped_mm._ext import DEV_BAD_OFFS, device_status
+
+    device_status()
+    a, b, offs, sa, sb, _ = _case(3, 128, 128, [10, 10, 10], "kn", 2)
+    good = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb)
+    bad = torch.tensor([10, 20, 5000], dtype=torch.int32, device="cuda")
+    assert torch.equal(fp8_block.grouped_mm_fp8_block(a, b, bad, sa, sb), good)
+    assert device_status() == DEV_BAD_OFFS
+
+
+def test_product_refusals():
+    from cutlass_op.bf16_grouped_mm import fp8_block
+
+    a, b, offs, sa, sb, bias = _case(2, 256, 256, [10, 10], "kn", 3)
+    f = fp8_block.grouped_mm_fp8_block
+    for args, words in [
+        ((a.float(), b, offs, sa, sb), "float8"),
+        ((a, b[:, :128], offs, sa, sb), "contraction"),
+        ((a, b[..., :250], offs, sa, sb), "multiple of 8"),
+        ((a, b, offs.long(), sa, sb), "int32"),
+        ((a, b, offs[:1], sa, sb), "int32"),
+        ((a, b, offs, sa[:, :1], sb), "scale_a"),
+        ((a, b, offs, sa.double(), sb), "scale_a"),
+        ((a, b, offs, sa.t().contiguous().t(), sb), "scale_a"),
+        ((a, b, offs, sa, sb[:, :, :1]), "scale_b"),
+        ((a, b, offs, sa, sb, bias.float()), "bias"),
+        ((a, b, offs, sa, sb, bias[:, :128]), "bias"),
+        ((a, b.cpu(), offs, sa, sb), "CUDA"),
+        ((a[:, 1:129], b[:, :128], offs, sa[:, :1], sb[:, :1]), "aligned"),
+    ]:
+        with pytest.raises(RuntimeError, match=words):
+            f(*args)
+    with pytest.raises(RuntimeError, match="multiple of 16"):
+        fp8_block.grouped_mm_swiglu_fp8_block(a, b[..., :248], offs, sa, sb, bias[:, :248].contiguous())
+    with pytest.raises(RuntimeError, match="aux"):
+        fp8_block.grouped_mm_swiglu_bwd_fp8_block(a, b, offs, torch.zeros(20, 256, device="cuda", dtype=torch.bfloat16),
+                                                  sa, sb)
