@@ -259,10 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
       uint32_t stage = 0, phase = 0;
-      uint32_t issued_parity[STAGES];
-      bool outstanding[STAGES];
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) { outstanding[s] = false; issued_parity[s] = 0; }
+      uint32_t issued = 0, issued_parity = 0;  // one bit per stage
       bool ok = true;
       for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
         const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
@@ -292,20 +289,20 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tma_load_3d(sB, &tmB, fb, kb * BK, nb0, ti.e);
             }
           }
-          outstanding[stage] = true;
-          issued_parity[stage] = phase;
+          issued |= 1u << stage;
+          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
       if (!ok && CG == 1) {
         // Stopped early: let the copies in flight land before the CTA exits (a pair meets at its barrier).
         for (int s = 0; s < STAGES; ++s)
-          if (outstanding[s])
-            wait_bounded(ptx::smem_u32(&full_bar[s]), issued_parity[s], abort_flag, p.status, kDrainLimitNs);
+          if ((issued >> s) & 1u)
+            wait_bounded(ptx::smem_u32(&full_bar[s]), (issued_parity >> s) & 1u, abort_flag, p.status, kDrainLimitNs);
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ UMMA issuer (even CTA)
+    // ------------------------------------------------------------ UMMA issuer (one thread of the even CTA)
     constexpr uint32_t idesc = ptx::make_idesc_e4m3(BM * CG, BN, false, B_MN);
     // MN-major B: 128-column chunks of 128 k rows, 16 KB apart, 32 k rows of 128 bytes per instruction;
     // K-major: 32 bytes of every 128-byte row per instruction
@@ -314,39 +311,37 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t a_kstep = 32u >> 4;
     uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, alternating TMEM buffers
     bool ok = true, issued_any = false;
-    if (leader) {
+    if (leader && lane == 0) {
       for (int t = unit; ok && t < total_tiles; t += num_units) {
         for (int kb = 0; kb < nk; ++kb, ++part) {
           const uint32_t buf = part & 1, bph = (part >> 1) & 1;
-          ok = __all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(&tempty_bar[buf]), bph ^ 1, abort_flag, p.status));
+          ok = wait_bounded(ptx::smem_u32(&tempty_bar[buf]), bph ^ 1, abort_flag, p.status);
           if (!ok) break;
-          ok = __all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status));
+          ok = wait_bounded(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status);
           if (!ok) break;
           ptx::tc_fence_after();
-          if (lane == 0) {
-            const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
-            const uint64_t adesc = ptx::make_smem_desc_sw128(sA, 16, 1024);
-            const uint64_t bdesc = ptx::make_smem_desc_sw128(sA + C::A_BYTES, b_lbo, 1024);
-            const uint32_t d_tmem = tmem_base + buf * BN;
+          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+          const uint64_t adesc = ptx::make_smem_desc_sw128(sA, 16, 1024);
+          const uint64_t bdesc = ptx::make_smem_desc_sw128(sA + C::A_BYTES, b_lbo, 1024);
+          const uint32_t d_tmem = tmem_base + buf * BN;
 #pragma unroll
-            for (int kk = 0; kk < kMmas; ++kk) {
-              if constexpr (CG == 2) ptx::umma_f8_pair(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
-              else ptx::umma_f8(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
-            }
-            if constexpr (CG == 2) {
-              ptx::umma_commit_pair(ptx::smem_u32(&empty_bar[stage]), 0x3);
-              ptx::umma_commit_pair(ptx::smem_u32(&tfull_bar[buf]), 0x3);
-            } else {
-              ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
-              ptx::umma_commit(ptx::smem_u32(&tfull_bar[buf]));
-            }
-            issued_any = true;
+          for (int kk = 0; kk < kMmas; ++kk) {
+            if constexpr (CG == 2) ptx::umma_f8_pair(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
+            else ptx::umma_f8(d_tmem, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, kk != 0);
           }
-          __syncwarp();
+          // the epilogue's signal first: the buffer's way round is the critical path
+          if constexpr (CG == 2) {
+            ptx::umma_commit_pair(ptx::smem_u32(&tfull_bar[buf]), 0x3);
+            ptx::umma_commit_pair(ptx::smem_u32(&empty_bar[stage]), 0x3);
+          } else {
+            ptx::umma_commit(ptx::smem_u32(&tfull_bar[buf]));
+            ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
+          }
+          issued_any = true;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok && lane == 0 && issued_any) {
+      if (!ok && issued_any) {
         // Stopped early: wait for the UMMAs already issued before TMEM is released.
         if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
         else ptx::umma_commit(ptx::smem_u32(drain_bar));

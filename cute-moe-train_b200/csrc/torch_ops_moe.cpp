@@ -48,6 +48,7 @@ int64_t row_stride(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : std::
 void check_matrix(const Tensor& t, const char* what, const char* name) {
   TORCH_CHECK(t.is_cuda(), what, ": ", name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == 2, what, ": ", name, " must be 2D, got ", t.dim(), "D");
+  if (t.numel() == 0) return;
   TORCH_CHECK(t.size(1) <= 1 || t.stride(1) == 1, what, ": ", name, " must have unit stride along its last dimension");
   TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= t.size(1), what, ": ", name, " must be row-major");
 }

@@ -122,3 +122,51 @@ def grouped_mm_swiglu_bwd_fp8_block(grad_output: torch.Tensor, down_w_t: torch.T
     with timed("fp8_block_down_dgrad_swiglu_bwd"):
         return torch.ops.grouped_mm.mm_swiglu_bwd_fp8_block(grad_output, down_w_t, offs, aux_biased_acc, scale_a,
                                                             scale_b, swiglu_alpha, swiglu_limit)
+
+
+class _FFNFp8Block(torch.autograd.Function):
+    """The MoE FFN with block-scaled e4m3 products and input gradients, bf16 weight gradients."""
+
+    @staticmethod
+    def forward(ctx, x, w_up, b_up, w_down, b_down, offs, alpha, limit, up_codes, down_codes):
+        q_up, s_up = up_codes if up_codes is not None else quantize_weights_block(w_up)
+        q_down, s_down = down_codes if down_codes is not None else quantize_weights_block(w_down)
+        qx, sx = quantize_rows_block(x)
+        s, aux = grouped_mm_swiglu_fp8_block(qx, q_up, offs, sx, s_up, b_up, alpha, limit)
+        qs, ss = quantize_rows_block(s)
+        out = grouped_mm_fp8_block(qs, q_down, offs, ss, s_down, b_down)
+        ctx.save_for_backward(x, s, aux, offs, q_up, s_up, q_down, s_down)
+        ctx.alpha, ctx.limit, ctx.has_b_down = alpha, limit, b_down is not None
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, s, aux, offs, q_up, s_up, q_down, s_down = ctx.saved_tensors
+        g = g.contiguous()
+        g_x = g_wu = g_bu = g_wd = g_bd = None
+        if ctx.needs_input_grad[3] or ctx.needs_input_grad[4]:
+            with timed("down_wgrad_bias"):
+                g_wd, g_bd = torch.ops.grouped_mm.mm_wgrad_bias(s.transpose(-2, -1), g, offs)
+        if any(ctx.needs_input_grad[:3]):
+            qg, sg = quantize_rows_block(g)
+            grad_aux = grouped_mm_swiglu_bwd_fp8_block(qg, q_down.transpose(1, 2), offs, aux, sg,
+                                                       s_down.transpose(1, 2), ctx.alpha, ctx.limit)
+            if ctx.needs_input_grad[0]:
+                qa, sa = quantize_rows_block(grad_aux)
+                g_x = grouped_mm_fp8_block(qa, q_up.transpose(1, 2), offs, sa, s_up.transpose(1, 2))
+            if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+                with timed("up_wgrad_bias"):
+                    g_wu, g_bu = torch.ops.grouped_mm.mm_wgrad_bias(x.transpose(-2, -1), grad_aux, offs)
+        return g_x, g_wu, g_bu, g_wd, g_bd if ctx.has_b_down else None, None, None, None, None, None
+
+
+def grouped_mm_ffn_fp8_block(x: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, offs: torch.Tensor,
+                             b_up: torch.Tensor, b_down: torch.Tensor | None = None, swiglu_alpha: float = 1.702,
+                             swiglu_limit: float = 7.0, up_codes: tuple[torch.Tensor, torch.Tensor] | None = None,
+                             down_codes: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+    """The MoE expert FFN of ``grouped_mm_ffn`` with block-scaled e4m3 forward products and input gradients;
+    bf16 inputs, parameters, output and gradients.  ``up_codes`` / ``down_codes``: the weights'
+    ``quantize_weights_block`` kept by the caller between optimizer steps (or for inference); quantised in
+    the call where absent.  The rows behind offs[-1] of the output (and of x's gradient) are not written."""
+    return _FFNFp8Block.apply(x, w_up, b_up, w_down, b_down, offs, swiglu_alpha, swiglu_limit, up_codes, down_codes)
