@@ -564,10 +564,10 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   if (g.epilogue < MGF_EPI_BIAS || g.epilogue > MGF_EPI_SWIGLU_BWD) return MGF_ERR_INVALID_ARGUMENT;
   if (g.total_rows < 0 || g.total_rows > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
   if (g.n <= 0 || g.k <= 0 || g.n > INT32_MAX / 2 || g.k > INT32_MAX / 2 || g.n % 8 != 0) return MGF_ERR_INVALID_ARGUMENT;
-  if (g.epilogue == MGF_EPI_SWIGLU && (g.n % 16 != 0 || g.d2 == nullptr || g.bias == nullptr))
-    return MGF_ERR_INVALID_ARGUMENT;
+  if (g.epilogue == MGF_EPI_SWIGLU && g.n % 16 != 0) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.total_rows == 0) return MGF_OK;  // nothing to write; the tensors of an empty batch have no address
+  if (g.epilogue == MGF_EPI_SWIGLU && (g.d2 == nullptr || g.bias == nullptr)) return MGF_ERR_INVALID_ARGUMENT;
   if (g.epilogue == MGF_EPI_SWIGLU_BWD && g.aux == nullptr) return MGF_ERR_INVALID_ARGUMENT;
-  if (g.total_rows == 0) return MGF_OK;
   if (g.a == nullptr || g.b == nullptr || g.offs == nullptr || g.scale_a == nullptr || g.scale_b == nullptr ||
       g.d == nullptr)
     return MGF_ERR_INVALID_ARGUMENT;
