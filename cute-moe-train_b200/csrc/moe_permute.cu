@@ -17,6 +17,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "moe_gemm.h"
 
@@ -37,10 +38,10 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortBatch = 4;  // ids loaded ahead per lane
 
 // One cluster of CTAs sorts all copies in one launch.  The copies are split into contiguous ranges, one
-// per warp; a warp ranks 32 copies at a time with match.any and keeps its own histogram in shared
-// memory, so the order within an expert is the copies' order.  Pass 1 counts, the histograms are
-// prefix-summed over the warps of a CTA, over the CTAs (distributed shared memory) and over the experts,
-// pass 2 walks the same ranges again and writes.
+// per warp, and every warp keeps its own histogram in shared memory.  Pass 1 counts (shared-memory
+// atomics: a count has no order), the histograms are prefix-summed over the warps of a CTA, over the
+// CTAs (distributed shared memory) and over the experts, pass 2 walks the same ranges again 32 copies at a
+// time, ranks them within the warp and writes, so the order within an expert is the copies' order.
 __device__ __forceinline__ int load_id(const int64_t* ids, int64_t i, int64_t end, int E, bool& bad) {
   if (i >= end) return -1;
   const int64_t v = __ldg(ids + i);
@@ -49,6 +50,20 @@ __device__ __forceinline__ int load_id(const int64_t* ids, int64_t i, int64_t en
     return -1;
   }
   return static_cast<int>(v);
+}
+
+// Lanes whose id equals this lane's (ids in [-1, 2^bits - 1)): one ballot per bit of id + 1.  A match.any gives
+// the same in one instruction, but its cost grows with the number of distinct ids in the warp: 98304
+// copies over 128 experts took 24 us with it.
+__device__ __forceinline__ unsigned same_id(int id, int bits) {
+  unsigned same = kFull;
+  const unsigned v = static_cast<unsigned>(id + 1);
+  for (int b = 0; b < bits; ++b) {
+    const bool bit = (v >> b) & 1u;
+    const unsigned set = __ballot_sync(kFull, bit);
+    same &= bit ? set : ~set;
+  }
+  return same;
 }
 
 __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
@@ -72,17 +87,15 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __res
   for (int i = threadIdx.x; i < kSortWarps * E; i += kSortThreads) hist[i] = 0;
   __syncthreads();
   int32_t* mine = hist + warp * E;
+  const int bits = 32 - __clz(E);  // of the largest id + 1
   bool bad = false;
   for (int64_t i = begin; i < end; i += 32 * kSortBatch) {
     int id[kSortBatch];
 #pragma unroll
     for (int b = 0; b < kSortBatch; ++b) id[b] = load_id(ids, i + 32 * b + lane, end, E, bad);
 #pragma unroll
-    for (int b = 0; b < kSortBatch; ++b) {
-      const unsigned same = __match_any_sync(kFull, id[b]);
-      if (id[b] >= 0 && lane == __ffs(same) - 1) mine[id[b]] += __popc(same);
-      __syncwarp();
-    }
+    for (int b = 0; b < kSortBatch; ++b)
+      if (id[b] >= 0) atomicAdd(mine + id[b], 1);
   }
   if (__any_sync(kFull, bad) && lane == 0) atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
   __syncthreads();
@@ -138,7 +151,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __res
 #pragma unroll
     for (int b = 0; b < kSortBatch; ++b) {
       const int64_t c = i + 32 * b + lane;
-      const unsigned same = __match_any_sync(kFull, id[b]);
+      const unsigned same = same_id(id[b], bits);
       int32_t row = -1;
       if (id[b] >= 0) row = base[id[b]] + mine[id[b]] + __popc(same & ((1u << lane) - 1u));
       __syncwarp();
@@ -157,44 +170,80 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __res
 }
 
 // ---------------------------------------------------------------- row access
-// V elements of 16 bytes (VEC) or one element at a time where a base, a pitch or the width is not a
-// multiple of 16 bytes.
+// 16 bytes (VEC) or one element at a time where a base, a pitch or the width is not a multiple of 16 bytes.
+// The raw words stay packed until they are added: unpacked early, the loads in flight would double the
+// registers and halve the warps that hide their latency.
 template <typename T, bool VEC>
 struct Access {
   static constexpr int N = VEC ? 16 / static_cast<int>(sizeof(T)) : 1;
-  struct Raw {
-    T v[N];
-  };
-  static __device__ __forceinline__ Raw load(const T* p) {
-    Raw r;
-    if constexpr (VEC) {
-      const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
-      *reinterpret_cast<uint4*>(r.v) = u;
-    } else {
-      r.v[0] = __ldg(p);
-    }
-    return r;
+  using Raw = typename std::conditional<VEC, uint4, T>::type;
+  static __device__ __forceinline__ Raw load(const T* p) { return __ldg(reinterpret_cast<const Raw*>(p)); }
+  static __device__ __forceinline__ void store(T* p, const Raw& r) { *reinterpret_cast<Raw*>(p) = r; }
+  static __device__ __forceinline__ Raw zero() {
+    if constexpr (VEC) return make_uint4(0, 0, 0, 0);
+    else return T(0.0f);
   }
-  static __device__ __forceinline__ void store(T* p, const Raw& r) {
-    if constexpr (VEC) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.v);
-    else p[0] = r.v[0];
+  // f[] = the elements of r in fp32
+  static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[N]) {
+    if constexpr (!VEC) {
+      f[0] = static_cast<float>(r);
+    } else {
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          f[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+          f[2 * i] = v.x;
+          f[2 * i + 1] = v.y;
+        } else {
+          f[2 * i] = __uint_as_float(w[i] << 16);
+          f[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+        }
+      }
+    }
+  }
+  // one rounding of every element
+  static __device__ __forceinline__ Raw pack(const float (&f)[N]) {
+    if constexpr (!VEC) {
+      return static_cast<T>(f[0]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, float>::value) {
+          w[i] = __float_as_uint(f[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+          const __half2 v = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        } else {
+          const __nv_bfloat162 v = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+          w[i] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+      return make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 };
 
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ void put(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half& d, float v) { d = __float2half_rn(v); }
-__device__ __forceinline__ void put(float& d, float v) { d = v; }
-
-__device__ __forceinline__ bool row_ok(int32_t r, int64_t n_rows, unsigned int* status) {
-  if (r < 0) return false;  // dropped copy
-  if (r >= n_rows) {        // a wrong plan: report it, touch nothing
-    atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
-    return false;
+// Rows of up to B copies of one token (-1: dropped, or outside the rows -- a wrong plan, which is reported
+// and touched nowhere).  All indices are loaded before the first is looked at: a check in between would
+// make every load wait for the one before it.
+template <int B>
+__device__ __forceinline__ void load_rows(const int32_t* row_of_copy, int count, int64_t n_rows, unsigned int* status,
+                                          int32_t (&row)[B]) {
+#pragma unroll
+  for (int b = 0; b < B; ++b) row[b] = b < count ? __ldg(row_of_copy + b) : -1;
+  bool bad = false;
+#pragma unroll
+  for (int b = 0; b < B; ++b) {
+    if (row[b] >= n_rows) {
+      bad = true;
+      row[b] = -1;
+    }
   }
-  return true;
+  if (bad) atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
 }
 
 // Zeros into the rows behind the last one, offs_end[0] .. n_rows, shared out over the whole grid.
@@ -204,9 +253,7 @@ __device__ __forceinline__ void zero_tail(T* rows, int64_t ld, int64_t n_rows, i
   if (kept < 0) kept = 0;
   if (kept >= n_rows) return;
   using A = Access<T, VEC>;
-  typename A::Raw z;
-#pragma unroll
-  for (int i = 0; i < A::N; ++i) put(z.v[i], 0.0f);
+  const typename A::Raw z = A::zero();
   const int64_t w0 = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   const int64_t nw = (static_cast<int64_t>(gridDim.x) * blockDim.x) >> 5;
   for (int64_t r = kept + w0; r < n_rows; r += nw)
@@ -231,22 +278,26 @@ __global__ void __launch_bounds__(32 * kWarps)
 #pragma unroll
     for (int i = 0; i < kPermuteVecs; ++i)
       if (v0 + 32 * i < nv) r[i] = A::load(x + t * ldx + (v0 + 32 * i) * A::N);
-    for (int j = 0; j < topk; ++j) {
-      const int32_t row = __ldg(row_of_copy + t * topk + j);
-      if (!row_ok(row, n_rows, status)) continue;
-      T* d = rows + static_cast<int64_t>(row) * ldr;
+    for (int j0 = 0; j0 < topk; j0 += 4) {
+      int32_t row[4];
+      load_rows(row_of_copy + t * topk + j0, topk - j0, n_rows, status, row);
 #pragma unroll
-      for (int i = 0; i < kPermuteVecs; ++i)
-        if (v0 + 32 * i < nv) A::store(d + (v0 + 32 * i) * A::N, r[i]);
+      for (int b = 0; b < 4; ++b) {
+        if (row[b] < 0) continue;
+        T* d = rows + static_cast<int64_t>(row[b]) * ldr;
+#pragma unroll
+        for (int i = 0; i < kPermuteVecs; ++i)
+          if (v0 + 32 * i < nv) A::store(d + (v0 + 32 * i) * A::N, r[i]);
+      }
     }
   }
   zero_tail<T, VEC>(rows, ldr, n_rows, nv, offs_end);
 }
 
 // ---------------------------------------------------------------- unpermute
-constexpr int kSumVecs = 2;   // vectors per lane and work unit
 constexpr int kSumBatch = 4;  // copies whose loads are in flight together
 
+// One vector per lane: 4 loads in flight and few registers, so that many warps are resident.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(32 * kWarps)
     unpermute_kernel(const T* __restrict__ rows, int64_t ldr, int64_t n_rows, int64_t tokens, int topk, int64_t nv,
@@ -257,48 +308,32 @@ __global__ void __launch_bounds__(32 * kWarps)
   const int64_t u = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
   if (u >= tokens * chunks) return;
   const int64_t t = u / chunks;
-  const int64_t v0 = (u - t * chunks) * (32 * kSumVecs) + lane;
-  float acc[kSumVecs][A::N];
+  const int64_t v = (u - t * chunks) * 32 + lane;
+  if (v >= nv) return;
+  float acc[A::N];
 #pragma unroll
-  for (int i = 0; i < kSumVecs; ++i)
-#pragma unroll
-    for (int c = 0; c < A::N; ++c) acc[i][c] = 0.0f;
+  for (int c = 0; c < A::N; ++c) acc[c] = 0.0f;
   for (int j0 = 0; j0 < topk; j0 += kSumBatch) {
     int32_t row[kSumBatch];
     float w[kSumBatch];
-    typename A::Raw r[kSumBatch][kSumVecs];
+    typename A::Raw r[kSumBatch];
+#pragma unroll
+    for (int b = 0; b < kSumBatch; ++b)
+      w[b] = weights != nullptr && j0 + b < topk ? __ldg(weights + t * topk + j0 + b) : 1.0f;
+    load_rows(row_of_copy + t * topk + j0, topk - j0, n_rows, status, row);
+#pragma unroll
+    for (int b = 0; b < kSumBatch; ++b)
+      if (row[b] >= 0) r[b] = A::load(rows + static_cast<int64_t>(row[b]) * ldr + v * A::N);
 #pragma unroll
     for (int b = 0; b < kSumBatch; ++b) {
-      row[b] = j0 + b < topk ? __ldg(row_of_copy + t * topk + j0 + b) : -1;
-      w[b] = weights != nullptr && j0 + b < topk ? __ldg(weights + t * topk + j0 + b) : 1.0f;
-      if (!row_ok(row[b], n_rows, status)) row[b] = -1;
+      if (row[b] < 0) continue;
+      float f[A::N];
+      A::unpack(r[b], f);
+#pragma unroll
+      for (int c = 0; c < A::N; ++c) acc[c] = fmaf(w[b], f[c], acc[c]);
     }
-#pragma unroll
-    for (int b = 0; b < kSumBatch; ++b)
-      if (row[b] >= 0) {
-#pragma unroll
-        for (int i = 0; i < kSumVecs; ++i)
-          if (v0 + 32 * i < nv) r[b][i] = A::load(rows + static_cast<int64_t>(row[b]) * ldr + (v0 + 32 * i) * A::N);
-      }
-#pragma unroll
-    for (int b = 0; b < kSumBatch; ++b)
-      if (row[b] >= 0) {
-#pragma unroll
-        for (int i = 0; i < kSumVecs; ++i)
-          if (v0 + 32 * i < nv) {
-#pragma unroll
-            for (int c = 0; c < A::N; ++c) acc[i][c] = fmaf(w[b], to_f(r[b][i].v[c]), acc[i][c]);
-          }
-      }
   }
-#pragma unroll
-  for (int i = 0; i < kSumVecs; ++i)
-    if (v0 + 32 * i < nv) {
-      typename A::Raw o;
-#pragma unroll
-      for (int c = 0; c < A::N; ++c) put(o.v[c], acc[i][c]);
-      A::store(out + t * ldo + (v0 + 32 * i) * A::N, o);
-    }
+  A::store(out + t * ldo + v * A::N, A::pack(acc));
 }
 
 // ---------------------------------------------------------------- unpermute, backward
@@ -324,13 +359,13 @@ __global__ void __launch_bounds__(32 * kWarps)
       float w[kBwdBatch], dot[kBwdBatch];
 #pragma unroll
       for (int b = 0; b < kBwdBatch; ++b) {
-        row[b] = j0 + b < topk ? __ldg(row_of_copy + t * topk + j0 + b) : -1;
-        if (!row_ok(row[b], n_rows, status)) row[b] = -1;
         w[b] = weights != nullptr && j0 + b < topk ? __ldg(weights + t * topk + j0 + b) : 1.0f;
         dot[b] = 0.0f;
       }
+      load_rows(row_of_copy + t * topk + j0, topk - j0, n_rows, status, row);
       for (int64_t v = sub * 32 + lane; v < nv; v += 32 * WPT) {
-        const typename A::Raw gv = A::load(g + t * ldg + v * A::N);
+        float gf[A::N];
+        A::unpack(A::load(g + t * ldg + v * A::N), gf);
         typename A::Raw rv[kBwdBatch];
         if (grad_weights != nullptr) {
 #pragma unroll
@@ -340,15 +375,16 @@ __global__ void __launch_bounds__(32 * kWarps)
 #pragma unroll
         for (int b = 0; b < kBwdBatch; ++b) {
           if (row[b] < 0) continue;
+          float f[A::N];
           if (grad_weights != nullptr) {
+            A::unpack(rv[b], f);
 #pragma unroll
-            for (int c = 0; c < A::N; ++c) dot[b] = fmaf(to_f(rv[b].v[c]), to_f(gv.v[c]), dot[b]);
+            for (int c = 0; c < A::N; ++c) dot[b] = fmaf(f[c], gf[c], dot[b]);
           }
           if (grad_rows != nullptr) {
-            typename A::Raw o;
 #pragma unroll
-            for (int c = 0; c < A::N; ++c) put(o.v[c], w[b] * to_f(gv.v[c]));
-            A::store(grad_rows + static_cast<int64_t>(row[b]) * ldgr + v * A::N, o);
+            for (int c = 0; c < A::N; ++c) f[c] = w[b] * gf[c];
+            A::store(grad_rows + static_cast<int64_t>(row[b]) * ldgr + v * A::N, A::pack(f));
           }
         }
       }
@@ -495,7 +531,7 @@ extern "C" int mgf_moe_unpermute(const void* rows, int32_t dtype, int64_t ldr, i
   return for_type(dtype, vec, [&](auto e, auto v) {
     using T = decltype(e);
     constexpr bool VEC = decltype(v)::value;
-    const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 32 * kSumVecs - 1) / (32 * kSumVecs);
+    const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 31) / 32;
     unsigned grid;
     if (!grid_of(tokens * chunks, grid)) return static_cast<int>(MGF_ERR_INVALID_ARGUMENT);
     unpermute_kernel<T, VEC><<<grid, 32 * kWarps, 0, static_cast<cudaStream_t>(stream)>>>(

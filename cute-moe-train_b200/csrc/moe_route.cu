@@ -13,7 +13,8 @@
 //
 // One warp per token, R = ceil(E / 32) logits per lane in registers.  The keys are mapped to unsigned
 // integers of the same order, so that one selection is a redux.sync maximum of the key and a redux.sync
-// minimum of the expert among the lanes that hold it.  Statistics and sums are fp32.  Each pass reads
+// minimum of the expert among the lanes that hold it; bf16 logits without a bias have 16-bit keys, and key
+// and expert go into one word and one maximum (PACKED).  Statistics and sums are fp32.  Each pass reads
 // the logits once and writes its outputs once; at the sizes of one step (24576 tokens, 128 experts: 6 MB)
 // launch and load latency bound it, not bandwidth.
 #include <cuda_bf16.h>
@@ -79,7 +80,7 @@ __device__ __forceinline__ float chosen_prob(float v, bool live, int score, bool
   return score == MGF_ROUTE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : expf(v - row_max) / row_sum;
 }
 
-template <typename T, int R>
+template <typename T, int R, bool PACKED>
 __global__ void __launch_bounds__(32 * kWarpsPerBlock)
     route_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int E, int topk, int score, bool renorm,
                  float scale, const float* __restrict__ bias, const uint8_t* __restrict__ token_mask,
@@ -103,6 +104,8 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
       const int e = lane + 32 * i;
       key[i] = order_key(bias != nullptr && e < E ? v[i] + __ldg(bias + e) : v[i]);
       if (v[i] == -INFINITY) key[i] = 0u;  // an expert masked in the logits stays masked under any bias
+      // the low half of a bf16 key says nothing; the earlier expert gets the larger word
+      if (PACKED && key[i] != 0u) key[i] = (key[i] & 0xffff0000u) | static_cast<uint32_t>(0xffff - e);
     }
     if (score == MGF_ROUTE_SOFTMAX && !renorm) {
       float m = v[0], s = 0.0f;
@@ -124,7 +127,8 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
         }
       const uint32_t top = __reduce_max_sync(kFull, best);
       if (top == 0u) break;  // nothing left to choose
-      const int e = static_cast<int>(__reduce_min_sync(kFull, best == top ? static_cast<uint32_t>(lane + 32 * at) : ~0u));
+      const int e = PACKED ? 0xffff - static_cast<int>(top & 0xffffu)
+                           : static_cast<int>(__reduce_min_sync(kFull, best == top ? static_cast<uint32_t>(lane + 32 * at) : ~0u));
       float ve = 0.0f;
 #pragma unroll
       for (int i = 0; i < R; ++i)
@@ -238,7 +242,10 @@ extern "C" int mgf_moe_route(const void* logits, int32_t dtype, int64_t ld, int6
   auto run = [&](auto tag) {
     using T = decltype(tag);
     return for_width<T>(num_experts, [&](auto r) {
-      route_kernel<T, decltype(r)::value><<<grid, 32 * kWarpsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(
+      constexpr int R = decltype(r)::value;
+      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+      auto kern = kBf16 && bias == nullptr ? route_kernel<T, R, kBf16> : route_kernel<T, R, false>;
+      kern<<<grid, 32 * kWarpsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(
           static_cast<const T*>(logits), ld, tokens, num_experts, topk, score, renormalize != 0, scale, bias,
           token_mask, weights, expert_idx);
       return cudaGetLastError() == cudaSuccess ? MGF_OK : MGF_ERR_CUDA;

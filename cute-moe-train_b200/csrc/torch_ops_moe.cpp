@@ -479,6 +479,7 @@ struct Route : torch::autograd::Function<Route> {
     ctx->saved_data["score"] = score;
     ctx->saved_data["renormalize"] = renormalize;
     ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);  // no zeros for the ids' missing gradient
     ctx->mark_non_differentiable({idx});
     return {weights, idx};
   }
@@ -509,6 +510,7 @@ struct Permute : torch::autograd::Function<Permute> {
     at::AutoDispatchBelowADInplaceOrView below;
     auto [rows, offs, row_of_copy, copy_of_row] = call_permute(x, idx, E);
     ctx->save_for_backward({offs, row_of_copy});
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({offs, row_of_copy, copy_of_row});
     return {rows, offs, row_of_copy, copy_of_row};
   }
