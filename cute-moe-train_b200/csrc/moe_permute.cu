@@ -16,6 +16,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <type_traits>
 
@@ -33,28 +34,29 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;  // warps per block of the row kernels
 
 // ---------------------------------------------------------------- sort
-constexpr int kSortThreads = 1024;
-constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortBatch = 4;  // ids loaded ahead per lane
+constexpr int kSortBatch = 8;  // ids a lane loads together (and keeps from pass 1 to pass 2)
 
 // One cluster of CTAs sorts all copies in one launch.  The copies are split into contiguous ranges, one
 // per warp, and every warp keeps its own histogram in shared memory.  Pass 1 counts (shared-memory
 // atomics: a count has no order), the histograms are prefix-summed over the warps of a CTA, over the
 // CTAs (distributed shared memory) and over the experts, pass 2 walks the same ranges again 32 copies at a
 // time, ranks them within the warp and writes, so the order within an expert is the copies' order.
-__device__ __forceinline__ int load_id(const int64_t* ids, int64_t i, int64_t end, int E, bool& bad) {
-  if (i >= end) return -1;
-  const int64_t v = __ldg(ids + i);
-  if (v >= E || v < -1) {
-    bad = true;
-    return -1;
+__device__ __forceinline__ void load_ids(const int64_t* ids, int64_t first, int64_t end, int E, int lane,
+                                         int (&id)[kSortBatch], bool& bad) {
+  int64_t v[kSortBatch];
+#pragma unroll
+  for (int b = 0; b < kSortBatch; ++b) v[b] = first + 32 * b + lane < end ? __ldg(ids + first + 32 * b + lane) : -1;
+#pragma unroll
+  for (int b = 0; b < kSortBatch; ++b) {
+    const bool ok = v[b] >= -1 && v[b] < E;
+    bad |= !ok;
+    id[b] = ok ? static_cast<int>(v[b]) : -1;
   }
-  return static_cast<int>(v);
 }
 
 // Lanes whose id equals this lane's (ids in [-1, 2^bits - 1)): one ballot per bit of id + 1.  A match.any gives
 // the same in one instruction, but its cost grows with the number of distinct ids in the warp: 98304
-// copies over 128 experts took 24 us with it.
+// copies over 128 experts took 24 us with it, 18 with ballots and the rest unchanged.
 __device__ __forceinline__ unsigned same_id(int id, int bits) {
   unsigned same = kFull;
   const unsigned v = static_cast<unsigned>(id + 1);
@@ -66,57 +68,71 @@ __device__ __forceinline__ unsigned same_id(int id, int bits) {
   return same;
 }
 
-__global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
-                                                            int32_t* __restrict__ offs,
-                                                            int32_t* __restrict__ row_of_copy,
-                                                            int32_t* __restrict__ copy_of_row,
-                                                            unsigned int* __restrict__ status) {
+// blockDim.x: a multiple of 32, at least E, at most 1024.
+__global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
+                                                    int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
+                                                    int32_t* __restrict__ copy_of_row,
+                                                    unsigned int* __restrict__ status) {
   extern __shared__ int32_t smem[];
-  int32_t* hist = smem;                     // [kSortWarps][E]
-  int32_t* total = smem + kSortWarps * E;   // [E] this CTA's counts, read by the other CTAs
-  int32_t* base = total + E;                // [E] first row of this CTA's copies of each expert
-  __shared__ int32_t warp_sums[kSortWarps];
+  const int threads = blockDim.x, warps = threads >> 5;
+  int32_t* hist = smem;                // [warps][E]
+  int32_t* total = smem + warps * E;   // [E] this CTA's counts, read by the other CTAs
+  int32_t* base = total + E;           // [E] first row of this CTA's copies of each expert
+  __shared__ int32_t warp_sums[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t units = static_cast<int64_t>(ctas) * kSortWarps;
+  const int64_t units = static_cast<int64_t>(ctas) * warps;
   const int64_t per = ((n + units - 1) / units + 31) / 32 * 32;
-  const int64_t unit = static_cast<int64_t>(rank) * kSortWarps + warp;
+  const int64_t unit = static_cast<int64_t>(rank) * warps + warp;
   const int64_t begin = unit * per < n ? unit * per : n;
   const int64_t end = begin + per < n ? begin + per : n;
-  for (int i = threadIdx.x; i < kSortWarps * E; i += kSortThreads) hist[i] = 0;
-  __syncthreads();
-  int32_t* mine = hist + warp * E;
   const int bits = 32 - __clz(E);  // of the largest id + 1
   bool bad = false;
-  for (int64_t i = begin; i < end; i += 32 * kSortBatch) {
-    int id[kSortBatch];
-#pragma unroll
-    for (int b = 0; b < kSortBatch; ++b) id[b] = load_id(ids, i + 32 * b + lane, end, E, bad);
+  int id[kSortBatch];
+  load_ids(ids, begin, end, E, lane, id, bad);
+  for (int i = threadIdx.x; i < warps * E; i += threads) hist[i] = 0;
+  if (threadIdx.x < 32) warp_sums[threadIdx.x] = 0;
+  __syncthreads();
+  int32_t* mine = hist + warp * E;
+  for (int64_t i = begin;;) {
 #pragma unroll
     for (int b = 0; b < kSortBatch; ++b)
       if (id[b] >= 0) atomicAdd(mine + id[b], 1);
+    i += 32 * kSortBatch;
+    if (i >= end) break;
+    load_ids(ids, i, end, E, lane, id, bad);
   }
   if (__any_sync(kFull, bad) && lane == 0) atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
   __syncthreads();
-  for (int e = threadIdx.x; e < E; e += kSortThreads) {
+  if (threadIdx.x < E) {
+    const int e = threadIdx.x;
     int32_t run = 0;
-#pragma unroll 8
-    for (int w = 0; w < kSortWarps; ++w) {
-      const int32_t c = hist[w * E + e];
-      hist[w * E + e] = run;
-      run += c;
+    for (int w0 = 0; w0 < warps; w0 += 8) {  // warps is 8, 16, 24 or 32
+      int32_t c[8];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) c[w] = hist[(w0 + w) * E + e];
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {
+        hist[(w0 + w) * E + e] = run;
+        run += c[w];
+      }
     }
     total[e] = run;
   }
-  cluster.sync();
-  // one expert per thread (E <= 1024 = kSortThreads): counts of all CTAs and of those before this one
+  if (ctas > 1) cluster.sync();
+  else __syncthreads();
+  // one expert per thread: counts of all CTAs and of those before this one
   int32_t all = 0, before = 0;
   if (threadIdx.x < E) {
-    for (int c = 0; c < ctas; ++c) {
-      const int32_t v = cluster.map_shared_rank(total, c)[threadIdx.x];
-      all += v;
-      before += c < rank ? v : 0;
+    if (ctas > 1) {
+      for (int c = 0; c < ctas; ++c) {
+        const int32_t v = cluster.map_shared_rank(total, c)[threadIdx.x];
+        all += v;
+        before += c < rank ? v : 0;
+      }
+    } else {
+      all = total[threadIdx.x];
     }
   }
   int32_t incl = all;
@@ -142,14 +158,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __res
     base[threadIdx.x] = first + before;
     if (rank == 0) offs[threadIdx.x] = first + all;
   }
-  const int32_t kept = warp_sums[kSortWarps - 1];
+  const int32_t kept = warp_sums[31];
   __syncthreads();
-  for (int64_t i = begin; i < end; i += 32 * kSortBatch) {
-    int id[kSortBatch];
-#pragma unroll
-    for (int b = 0; b < kSortBatch; ++b) id[b] = load_id(ids, i + 32 * b + lane, end, E, bad);
+  if (end - begin > 32 * kSortBatch) load_ids(ids, begin, end, E, lane, id, bad);  // else the registers still hold them
+  for (int64_t i = begin; i < end;) {
 #pragma unroll
     for (int b = 0; b < kSortBatch; ++b) {
+      if (i + 32 * b >= end) break;  // the same for all lanes
       const int64_t c = i + 32 * b + lane;
       const unsigned same = same_id(id[b], bits);
       int32_t row = -1;
@@ -162,11 +177,13 @@ __global__ void __launch_bounds__(kSortThreads) sort_kernel(const int64_t* __res
         if (row >= 0) copy_of_row[row] = static_cast<int32_t>(c);
       }
     }
+    i += 32 * kSortBatch;
+    if (i < end) load_ids(ids, i, end, E, lane, id, bad);
   }
-  for (int64_t r = kept + static_cast<int64_t>(rank) * kSortThreads + threadIdx.x; r < n;
-       r += static_cast<int64_t>(ctas) * kSortThreads)
+  for (int64_t r = kept + static_cast<int64_t>(rank) * threads + threadIdx.x; r < n;
+       r += static_cast<int64_t>(ctas) * threads)
     copy_of_row[r] = -1;
-  cluster.sync();  // no CTA leaves while another may still read its counts
+  if (ctas > 1) cluster.sync();  // no CTA leaves while another may still read its counts
 }
 
 // ---------------------------------------------------------------- row access
@@ -467,16 +484,24 @@ extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_ex
     return MGF_ERR_INVALID_ARGUMENT;
   unsigned int* status = status_word_address();
   if (status == nullptr) return MGF_ERR_CUDA;
-  const size_t smem = static_cast<size_t>(kSortWarps + 2) * num_experts * sizeof(int32_t);
-  if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>((kSortWarps + 2) * 1024 * sizeof(int32_t))) != cudaSuccess)
-    return MGF_ERR_CUDA;
-  // one CTA up to four batches per warp, then 2, 4 and 8 (the portable cluster size)
-  const int64_t per_cta = static_cast<int64_t>(kSortThreads) * kSortBatch;
-  const unsigned ctas = n <= per_cta ? 1 : n <= 2 * per_cta ? 2 : n <= 4 * per_cta ? 4 : 8;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MGF_ERR_CUDA;
+  static std::atomic<bool> attr_done[64];
+  if (!attr_done[dev]) {
+    if (cudaFuncSetAttribute(sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             static_cast<int>(34 * 1024 * sizeof(int32_t))) != cudaSuccess)
+      return MGF_ERR_CUDA;
+    attr_done[dev] = true;
+  }
+  // few copies: 8 warps (as many as E needs threads); then one CTA of 32 warps up to 128 copies per warp, then
+  // 2, 4 and 8 CTAs (the portable cluster size)
+  const unsigned least = (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
+  const unsigned threads = n <= 1024 ? least : 1024u;
+  const unsigned ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
+  const size_t smem = static_cast<size_t>(threads / 32 + 2) * num_experts * sizeof(int32_t);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(kSortThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
