@@ -20,6 +20,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -77,7 +78,23 @@ struct Params {
   int aux_v8, d_v8, d2_v8;  // base 32-byte aligned and row pitch a multiple of 32 bytes
   int stall_test;           // test hook: no tile is loaded, so every consumer wait runs out
   unsigned int* status;
+  // The form with the scales in the tensor cores (below) runs where every scale is a power of two, the form with
+  // the promotion in registers where one is not: pack_scales_kernel leaves one word per block, not 0 where it
+  // found another number, and each form returns at once where the words call for the other.  nullptr: no choice.
+  const int32_t* other_scales;
+  int num_words;
+  // packed scales: byte j of a word is the exponent of block 4 * w + j; [w][row] and [e][w][n block]
+  const uint32_t* packed_a;
+  const uint32_t* packed_b;
+  int64_t packed_rows;  // row pitch of packed_a: rows past the last one that a tile reads included
 };
+
+// Whether some scale is no power of two; one barrier, all threads of the CTA.
+__device__ __forceinline__ bool any_other_scale(const Params& p) {
+  int found = 0;
+  for (int i = threadIdx.x; i < p.num_words; i += blockDim.x) found |= __ldg(p.other_scales + i);
+  return __syncthreads_or(found) != 0;
+}
 
 struct Tile {
   int e, n0, row0, row_end;
@@ -186,10 +203,76 @@ __device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, floa
   return pack_bf16x2(d_gate, d_up);
 }
 
+// Epilogue of one row's COLS columns from column c0 on.
+template <int EPI, int COLS>
+__device__ __forceinline__ void write_columns(const Params& p, const float (&acc)[COLS], int e, int grow, int c0) {
+  // 32 columns at a time; n is a multiple of 8 (SWIGLU: 16), so units of 8 columns are whole
+#pragma unroll
+  for (int c = 0; c < COLS / 32; ++c) {
+    const int col0 = c0 + c * 32;
+    if (col0 >= p.n) break;
+    if constexpr (EPI == MGF_EPI_SWIGLU_BWD) {
+      uint4 aw[8];
+      load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0, p.n, true, p.aux_v8, aw);
+      uint4* gp = reinterpret_cast<uint4*>(p.d + (int64_t)grow * p.ldd + 2 * col0);
+      const int nvalid = (p.n - col0) >> 2;
+#pragma unroll
+      for (int g = 0; g < 8; g += 2) {
+        if (g < nvalid) {
+          uint4 o[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* f = acc + c * 32 + 4 * (g + h);
+            o[h].x = swiglu_bwd(f[0], aw[g + h].x, p.alpha, p.limit);
+            o[h].y = swiglu_bwd(f[1], aw[g + h].y, p.alpha, p.limit);
+            o[h].z = swiglu_bwd(f[2], aw[g + h].z, p.alpha, p.limit);
+            o[h].w = swiglu_bwd(f[3], aw[g + h].w, p.alpha, p.limit);
+          }
+          if (p.d_v8) ptx::st_v8(gp + g, o[0], o[1]);
+          else {
+            gp[g] = o[0];
+            gp[g + 1] = o[1];
+          }
+        }
+      }
+    } else {
+      uint32_t packed[16];
+      const uint4* bp = reinterpret_cast<const uint4*>(p.bias + (int64_t)e * p.bias_stride + col0);
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint4 b = make_uint4(0, 0, 0, 0);
+        if (p.bias != nullptr && col0 + 8 * g < p.n) b = __ldg(bp + g);
+        const uint32_t w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          const float* f = acc + c * 32 + 8 * g + 2 * h;
+          packed[4 * g + h] = pack_bf16x2(f[0] + bf16_lo(w[h]), f[1] + bf16_hi(w[h]));
+        }
+      }
+      uint4 u[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        u[g] = make_uint4(packed[4 * g], packed[4 * g + 1], packed[4 * g + 2], packed[4 * g + 3]);
+      store_units<4>(p.d + (int64_t)grow * p.ldd + col0, u, (p.n - col0) >> 3, p.d_v8);
+      if constexpr (EPI == MGF_EPI_SWIGLU) {
+        uint32_t so[8];
+#pragma unroll
+        for (int h = 0; h < 8; ++h)
+          so[h] = pack_bf16x2(
+              swiglu(bf16_lo(packed[2 * h]), bf16_hi(packed[2 * h]), p.alpha, p.limit),
+              swiglu(bf16_lo(packed[2 * h + 1]), bf16_hi(packed[2 * h + 1]), p.alpha, p.limit));
+        const uint4 us[2] = {make_uint4(so[0], so[1], so[2], so[3]), make_uint4(so[4], so[5], so[6], so[7])};
+        store_units<2>(p.d2 + (int64_t)grow * p.ldd2 + (col0 >> 1), us, (p.n - col0) >> 4, p.d2_v8);
+      }
+    }
+  }
+}
+
 template <int BN, int EPI, bool B_MN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
   using C = Cfg<BN, CG>;
+  if (p.other_scales != nullptr && !any_other_scale(p)) return;
   constexpr int STAGES = C::STAGES;
   constexpr int TM = BM * CG;       // rows of a tile
   constexpr int COLS = BN / 2;      // columns of a tile that one epilogue thread owns
@@ -402,66 +485,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (!valid || !active) continue;
-      // 32 columns at a time; n is a multiple of 8 (SWIGLU: 16), so units of 8 columns are whole
-#pragma unroll
-      for (int c = 0; c < COLS / 32; ++c) {
-        const int col0 = c0 + c * 32;
-        if (col0 >= p.n) break;
-        if constexpr (EPI == MGF_EPI_SWIGLU_BWD) {
-          uint4 aw[8];
-          load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0, p.n, true, p.aux_v8, aw);
-          uint4* gp = reinterpret_cast<uint4*>(p.d + (int64_t)grow * p.ldd + 2 * col0);
-          const int nvalid = (p.n - col0) >> 2;
-#pragma unroll
-          for (int g = 0; g < 8; g += 2) {
-            if (g < nvalid) {
-              uint4 o[2];
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const float* f = acc + c * 32 + 4 * (g + h);
-                o[h].x = swiglu_bwd(f[0], aw[g + h].x, p.alpha, p.limit);
-                o[h].y = swiglu_bwd(f[1], aw[g + h].y, p.alpha, p.limit);
-                o[h].z = swiglu_bwd(f[2], aw[g + h].z, p.alpha, p.limit);
-                o[h].w = swiglu_bwd(f[3], aw[g + h].w, p.alpha, p.limit);
-              }
-              if (p.d_v8) ptx::st_v8(gp + g, o[0], o[1]);
-              else {
-                gp[g] = o[0];
-                gp[g + 1] = o[1];
-              }
-            }
-          }
-        } else {
-          uint32_t packed[16];
-          const uint4* bp = reinterpret_cast<const uint4*>(p.bias + (int64_t)ti.e * p.bias_stride + col0);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint4 b = make_uint4(0, 0, 0, 0);
-            if (p.bias != nullptr && col0 + 8 * g < p.n) b = __ldg(bp + g);
-            const uint32_t w[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int h = 0; h < 4; ++h) {
-              const float* f = acc + c * 32 + 8 * g + 2 * h;
-              packed[4 * g + h] = pack_bf16x2(f[0] + bf16_lo(w[h]), f[1] + bf16_hi(w[h]));
-            }
-          }
-          uint4 u[4];
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            u[g] = make_uint4(packed[4 * g], packed[4 * g + 1], packed[4 * g + 2], packed[4 * g + 3]);
-          store_units<4>(p.d + (int64_t)grow * p.ldd + col0, u, (p.n - col0) >> 3, p.d_v8);
-          if constexpr (EPI == MGF_EPI_SWIGLU) {
-            uint32_t so[8];
-#pragma unroll
-            for (int h = 0; h < 8; ++h)
-              so[h] = pack_bf16x2(
-                  swiglu(bf16_lo(packed[2 * h]), bf16_hi(packed[2 * h]), p.alpha, p.limit),
-                  swiglu(bf16_lo(packed[2 * h + 1]), bf16_hi(packed[2 * h + 1]), p.alpha, p.limit));
-            const uint4 us[2] = {make_uint4(so[0], so[1], so[2], so[3]), make_uint4(so[4], so[5], so[6], so[7])};
-            store_units<2>(p.d2 + (int64_t)grow * p.ldd2 + (col0 >> 1), us, (p.n - col0) >> 4, p.d2_v8);
-          }
-        }
-      }
+      write_columns<EPI, COLS>(p, acc, ti.e, grow, c0);
     }
   }
 
@@ -474,6 +498,295 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (CG == 2) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
     else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
+}
+
+// ---------------------------------------------------------------- scales in the tensor cores
+// Where all scales are powers of two (what the quantisers make), the tensor cores apply them: kind::mxf8f6f4 takes a
+// power-of-two scale per row of A and column of B for every 32 elements of k, here the same one four times.
+// The accumulator then stays in TMEM over the whole contraction and no promotion is needed.
+
+// Scales as bytes, and whether there is one that is no power of two.  A: rows of groups only (those behind the
+// last group have no result, and moe_permute_fp8 gives them zeros).  One thread per row, four blocks at a time.
+__global__ void __launch_bounds__(256) pack_scales_kernel(const Params p, uint32_t* __restrict__ pa,
+                                                          uint32_t* __restrict__ pb, int32_t* __restrict__ words) {
+  const int nk = (p.k + BK - 1) / BK, nkw = (nk + 3) / 4, nnb = (p.n + BK - 1) / BK;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int64_t nt = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  bool other = false;
+  auto byte_of = [&](float s) -> uint32_t {
+    const uint32_t b = __float_as_uint(s), e = b >> 23;
+    other |= (b & 0x807FFFFFu) != 0u || e == 0u || e == 255u;
+    return e & 0xffu;
+  };
+  int64_t rows = __ldg(p.offs + p.E - 1);
+  rows = rows < 0 ? 0 : (rows > p.total_rows ? p.total_rows : rows);
+  const bool vec = (reinterpret_cast<uintptr_t>(p.scale_a) & 15u) == 0 && p.lds_a % 4 == 0;
+  for (int64_t r = t0; r < rows; r += nt) {
+    const float* s = p.scale_a + r * p.lds_a;
+    for (int w = 0; w < nkw; ++w) {
+      uint32_t v = 0;
+      if (vec && 4 * w + 4 <= nk) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(s + 4 * w));
+        v = byte_of(f.x) | (byte_of(f.y) << 8) | (byte_of(f.z) << 16) | (byte_of(f.w) << 24);
+      } else {
+        for (int j = 0; j < 4; ++j)
+          if (4 * w + j < nk) v |= byte_of(__ldg(s + 4 * w + j)) << (8 * j);
+      }
+      pa[w * p.packed_rows + r] = v;
+    }
+  }
+  const int64_t nb = static_cast<int64_t>(p.E) * nkw * nnb;
+  for (int64_t i = t0; i < nb; i += nt) {
+    const int64_t c = i % nnb, w = i / nnb % nkw, e = i / nnb / nkw;
+    uint32_t v = 0;
+    for (int j = 0; j < 4; ++j)
+      if (4 * w + j < nk) v |= byte_of(__ldg(p.scale_b + e * p.sb_e + (4 * w + j) * p.sb_k + c * p.sb_n)) << (8 * j);
+    pb[i] = v;
+  }
+  const int found = __syncthreads_or(other ? 1 : 0);
+  if (threadIdx.x == 0) words[blockIdx.x] = found;
+}
+
+// TMEM: the accumulator's 256 columns, then kSlots scale slots of 4 columns (A: one word per row of 32 x 4) and of 8
+// (B: one word per column of 32 x 8).  One accumulator: the epilogue takes it into registers and hands it back before
+// it converts and stores, so that the next tile's products run under the stores.
+struct MxCfg {
+  static constexpr int BN = 256;
+  static constexpr int STAGE_BYTES = BM * BK + BN * BK;
+  static constexpr int STAGES = 4;
+  static constexpr int kSlots = 4;               // each holds the scales of four blocks of k
+  static constexpr int SLOT_BYTES = 512 + 1024;  // 128 rows of A, 256 columns of B
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SCHED_BYTES = 3 * 4 * (kMaxGroups + 1);
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + kSlots * SLOT_BYTES + BAR_BYTES + SCHED_BYTES;
+  static constexpr int TMEM_COLS = 512, SFA_COL = BN, SFB_COL = BN + 4 * kSlots;
+  static constexpr int kThreads = 384;  // producer, issuer, scales, schedule; 8 epilogue warps
+  static_assert(SMEM_BYTES <= 227 * 1024 && SFB_COL + 8 * kSlots <= TMEM_COLS, "shared and tensor memory");
+};
+
+template <int EPI, bool B_MN>
+__global__ void __launch_bounds__(MxCfg::kThreads, 1)
+    mx_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+  using C = MxCfg;
+  constexpr int STAGES = C::STAGES, BN = C::BN, COLS = BN / 2, kSlots = C::kSlots;
+  if (any_other_scale(p)) return;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* slots = smem + STAGES * C::STAGE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(slots + kSlots * C::SLOT_BYTES);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + STAGES;
+  uint64_t* sf_full = bars + 2 * STAGES;
+  uint64_t* sf_empty = bars + 2 * STAGES + kSlots;
+  uint64_t* tfull_bar = bars + 2 * STAGES + 2 * kSlots;
+  uint64_t* tempty_bar = tfull_bar + 1;
+  uint64_t* drain_bar = tfull_bar + 2;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull_bar + 3);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  int* prefix = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES);
+  int* seg_start = prefix + (kMaxGroups + 1);
+  int* seg_end = seg_start + (kMaxGroups + 1);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
+    }
+    for (int s = 0; s < kSlots; ++s) {
+      ptx::mbar_init(ptx::smem_u32(&sf_full[s]), 32);
+      ptx::mbar_init(ptx::smem_u32(&sf_empty[s]), 1);
+    }
+    ptx::mbar_init(ptx::smem_u32(tfull_bar), 1);
+    ptx::mbar_init(ptx::smem_u32(tempty_bar), kNumEpiWarps);
+    ptx::mbar_init(ptx::smem_u32(drain_bar), 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::prefetch_tmap(&tmA);
+    ptx::prefetch_tmap(&tmB);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
+    ptx::tmem_relinquish();
+  }
+  if (warp == 3) build_schedule<BM>(p, prefix, seg_start, seg_end, lane);
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem_base = *tmem_holder;
+  const int total_tiles = prefix[p.E];
+  const int nk = (p.k + BK - 1) / BK, nkw = (nk + 3) / 4, nnb = (p.n + BK - 1) / BK;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      uint32_t stage = 0, phase = 0;
+      uint32_t issued = 0, issued_parity = 0;  // one bit per stage
+      bool ok = true;
+      for (int t = blockIdx.x; ok && t < total_tiles && !p.stall_test; t += gridDim.x) {
+        const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
+        for (int kb = 0; kb < nk; ++kb) {
+          if (!wait_bounded(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status)) { ok = false; break; }
+          const uint32_t fb = ptx::smem_u32(&full_bar[stage]);
+          ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + BM * BK;
+          ptx::tma_load_2d(sA, &tmA, fb, kb * BK, ti.row0);
+          if constexpr (B_MN) {
+            ptx::tma_load_3d(sB, &tmB, fb, ti.n0, kb * BK, ti.e);
+            ptx::tma_load_3d(sB + 16384, &tmB, fb, ti.n0 + 128, kb * BK, ti.e);
+          } else {
+            ptx::tma_load_3d(sB, &tmB, fb, kb * BK, ti.n0, ti.e);
+          }
+          issued |= 1u << stage;
+          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+        }
+      }
+      if (!ok) {  // stopped early: let the copies in flight land before the CTA exits
+        for (int s = 0; s < STAGES; ++s)
+          if ((issued >> s) & 1u)
+            wait_bounded(ptx::smem_u32(&full_bar[s]), (issued_parity >> s) & 1u, abort_flag, p.status, kDrainLimitNs);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ UMMA issuer (one thread)
+    if (lane == 0) {
+      constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
+      constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
+      constexpr uint32_t a_kstep = 32u >> 4;
+      uint32_t stage = 0, phase = 0, slot = 0, sphase = 0, tphase = 0;
+      bool ok = true, issued_any = false;
+      for (int t = blockIdx.x; ok && t < total_tiles; t += gridDim.x, tphase ^= 1) {
+        ok = wait_bounded(ptx::smem_u32(tempty_bar), tphase ^ 1, abort_flag, p.status);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        uint32_t sfa = 0, sfb = 0;
+        for (int kb = 0; kb < nk; ++kb) {
+          if ((kb & 3) == 0) {  // the scales of the next four blocks
+            ok = wait_bounded(ptx::smem_u32(&sf_full[slot]), sphase, abort_flag, p.status);
+            if (!ok) break;
+            const uint32_t src = ptx::smem_u32(slots + slot * C::SLOT_BYTES);
+            sfa = tmem_base + C::SFA_COL + 4 * slot;
+            sfb = tmem_base + C::SFB_COL + 8 * slot;
+            ptx::tmem_cp_32x128b_x4(sfa, ptx::make_smem_desc_plain(src, 16, 128));
+            ptx::tmem_cp_32x128b_x4(sfb, ptx::make_smem_desc_plain(src + 512, 16, 128));
+            ptx::tmem_cp_32x128b_x4(sfb + 4, ptx::make_smem_desc_plain(src + 1024, 16, 128));
+          }
+          ok = wait_bounded(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status);
+          if (!ok) break;
+          ptx::tc_fence_after();
+          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
+          const uint64_t adesc = ptx::make_smem_desc_sw128(sA, 16, 1024);
+          const uint64_t bdesc = ptx::make_smem_desc_sw128(sA + BM * BK, b_lbo, 1024);
+          const uint32_t idesc = ptx::make_idesc_mxf8(BM, BN, false, B_MN, kb & 3);
+#pragma unroll
+          for (int kk = 0; kk < BK / 32; ++kk)
+            ptx::umma_mxf8(tmem_base, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, sfa, sfb, (kb | kk) != 0);
+          issued_any = true;
+          ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
+          if (++stage == STAGES) { stage = 0; phase ^= 1; }
+          if ((kb & 3) == 3 || kb == nk - 1) {
+            ptx::umma_commit(ptx::smem_u32(&sf_empty[slot]));
+            if (++slot == kSlots) { slot = 0; sphase ^= 1; }
+          }
+        }
+        if (!ok) break;
+        ptx::umma_commit(ptx::smem_u32(tfull_bar));
+      }
+      if (!ok && issued_any) {  // stopped early: wait for the UMMAs already issued before TMEM is released
+        ptx::umma_commit(ptx::smem_u32(drain_bar));
+        wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, p.status, kDrainLimitNs);
+      }
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ scales to shared memory, four blocks of k at a time
+    // tcgen05.cp takes 32 rows of 16 bytes: lane i's are the words of rows i, i + 32, i + 64 and i + 96 (of the
+    // columns for B, which within one block of 128 are all the same word).
+    uint32_t slot = 0, sphase = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; ok && t < total_tiles && !p.stall_test; t += gridDim.x) {
+      const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
+      const uint32_t* pa = p.packed_a + ti.row0 + lane;
+      const int c0 = ti.n0 / BK, c1 = c0 + 1 < nnb ? c0 + 1 : c0;
+      const uint32_t* pb = p.packed_b + static_cast<int64_t>(ti.e) * nkw * nnb;
+      for (int w = 0; w < nkw; ++w) {
+        const uint4 a = make_uint4(__ldg(pa + w * p.packed_rows), __ldg(pa + w * p.packed_rows + 32),
+                                   __ldg(pa + w * p.packed_rows + 64), __ldg(pa + w * p.packed_rows + 96));
+        const uint32_t b0 = __ldg(pb + w * nnb + c0), b1 = __ldg(pb + w * nnb + c1);
+        ok = __all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(&sf_empty[slot]), sphase ^ 1, abort_flag, p.status));
+        if (!ok) break;
+        uint4* dst = reinterpret_cast<uint4*>(slots + slot * C::SLOT_BYTES) + lane;
+        dst[0] = a;
+        dst[32] = make_uint4(b0, b0, b0, b0);
+        dst[64] = make_uint4(b1, b1, b1, b1);
+        ptx::fence_proxy_async_smem();
+        ptx::mbar_arrive(ptx::smem_u32(&sf_full[slot]));
+        if (++slot == kSlots) { slot = 0; sphase ^= 1; }
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ epilogue
+    const int q = warp & 3, wg = (warp - 4) >> 2;
+    uint32_t tphase = 0;
+    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, tphase ^= 1) {
+      const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
+      const int c0 = ti.n0 + wg * COLS, grow = ti.row0 + q * 32 + lane;
+      const bool active = ti.row0 + q * 32 < ti.row_end && c0 < p.n;  // warp-uniform
+      if (!__all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(tfull_bar), tphase, abort_flag, p.status))) break;
+      ptx::tc_fence_after();
+      float acc[COLS];
+      if (active) {
+        const uint32_t tb = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + wg * COLS;
+#pragma unroll
+        for (int c = 0; c < COLS / 32; ++c)
+          ptx::tmem_ld_32x32b_x32(tb + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&acc[c * 32]));
+        ptx::tmem_ld_wait();
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) arrive_relaxed(ptx::smem_u32(tempty_bar));
+      if (active && grow < ti.row_end) write_columns<EPI, COLS>(p, acc, ti.e, grow, c0);
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
+  }
+}
+
+template <int EPI, bool B_MN>
+int launch_mx(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
+  auto kern = mx_kernel<EPI, B_MN>;
+  static std::atomic<bool> attr_done[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MGF_ERR_CUDA;
+  if (!attr_done[dev]) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MxCfg::SMEM_BYTES);
+    if (e != cudaSuccess) {
+      record_error("cudaFuncSetAttribute", e);
+      return MGF_ERR_CUDA;
+    }
+    attr_done[dev] = true;
+  }
+  const unsigned grid = static_cast<unsigned>(tiles < sms ? tiles : sms);
+  cudaGetLastError();
+  kern<<<grid, MxCfg::kThreads, MxCfg::SMEM_BYTES, st>>>(tA, tB, p);
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess && debug_sync()) {
+    e = cudaStreamSynchronize(st);
+    fprintf(stderr, "[mgf] block-scaled mx epi=%d b_mn=%d grid=%u E=%d rows=%lld n=%d k=%d -> %s\n", EPI, int(B_MN), grid,
+            p.E, (long long)p.total_rows, p.n, p.k, cudaGetErrorString(e));
+  }
+  if (e != cudaSuccess) {
+    record_error("kernel launch", e);
+    return MGF_ERR_CUDA;
+  }
+  return MGF_OK;
 }
 
 template <int BN, int EPI, bool B_MN, int CG>
@@ -548,12 +861,56 @@ int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, c
   }
 }
 
+int dispatch_mx(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+                cudaStream_t st) {
+  switch (epi) {
+    case MGF_EPI_BIAS:
+      return b_mn ? launch_mx<MGF_EPI_BIAS, true>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_BIAS, false>(tA, tB, p, tiles, sms, st);
+    case MGF_EPI_SWIGLU:
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU, true>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU, false>(tA, tB, p, tiles, sms, st);
+    default:
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU_BWD, true>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU_BWD, false>(tA, tB, p, tiles, sms, st);
+  }
+}
+
+// Workspace of the form with the scales in the tensor cores: packed scales of A (128 rows past the end: a tile reads
+// whole 128-row blocks), of B, and a word per block of the packing kernel.
+constexpr int kPackBlocks = 296;
+struct MxSpace {
+  int64_t rows, a_words, b_words;
+  int64_t bytes() const { return 4 * (a_words + b_words + kPackBlocks); }
+};
+MxSpace mx_space(const mgf_block_gemm_desc& g) {
+  const int64_t nkw = ((g.k + BK - 1) / BK + 3) / 4, nnb = (g.n + BK - 1) / BK;
+  MxSpace s;
+  s.rows = (g.total_rows + BM + 3) / 4 * 4;
+  s.a_words = nkw * s.rows;
+  s.b_words = g.num_groups * nkw * nnb;
+  return s;
+}
+
+// The tensor cores' scales save the promotion but cost two small launches (packing; the form that returns at
+// once).  MGF_BLOCK_MX=0|1 forces a choice.
+bool use_mx(const mgf_block_gemm_desc& g) {
+  if (const char* env = getenv("MGF_BLOCK_MX"); env != nullptr && (env[0] == '0' || env[0] == '1')) return env[0] == '1';
+  return g.n > 128 && g.total_rows >= 1024;
+}
+
 bool aligned(const void* ptr, unsigned n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1u)) == 0; }
 
 }  // namespace block_gemm
 }  // namespace mgf
 
 extern "C" size_t mgf_block_gemm_desc_size(void) { return sizeof(mgf_block_gemm_desc); }
+
+extern "C" int64_t mgf_block_gemm_workspace_bytes(const mgf_block_gemm_desc* desc) {
+  using namespace mgf::block_gemm;
+  if (desc == nullptr || desc->num_groups < 1 || desc->total_rows <= 0 || desc->n <= 0 || desc->k <= 0) return 0;
+  return use_mx(*desc) ? mx_space(*desc).bytes() : 0;
+}
 
 extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stream) {
   using namespace mgf;
@@ -649,6 +1006,29 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   int sms = di.sms - (g.sm_carveout > 0 ? g.sm_carveout : 0);
   if (sms < cg) sms = cg;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (use_mx(g) && g.workspace != nullptr) {
+    if (!aligned(g.workspace, 16)) return MGF_ERR_ALIGNMENT;
+    const MxSpace sp = mx_space(g);
+    uint32_t* ws = static_cast<uint32_t*>(g.workspace);
+    int32_t* words = reinterpret_cast<int32_t*>(ws + sp.a_words + sp.b_words);
+    p.packed_a = ws;
+    p.packed_b = ws + sp.a_words;
+    p.packed_rows = sp.rows;
+    p.other_scales = words;
+    p.num_words = kPackBlocks;
+    pack_scales_kernel<<<kPackBlocks, 256, 0, st>>>(p, ws, ws + sp.a_words, words);
+    if (cudaGetLastError() != cudaSuccess) return MGF_ERR_CUDA;
+    Params pm = p;
+    pm.n_tiles = static_cast<int>((g.n + MxCfg::BN - 1) / MxCfg::BN);
+    CUtensorMap tBm;
+    const uint32_t bBm[3] = {BK, MxCfg::BN, 1};
+    if (!encode_bf16(&tBm, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bBm, CU_TENSOR_MAP_SWIZZLE_128B, u8))
+      return MGF_ERR_CUDA;
+    const int64_t mx_tiles = (g.total_rows / BM + g.num_groups) * static_cast<int64_t>(pm.n_tiles);
+    if (mx_tiles > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
+    const int rc = dispatch_mx(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st);
+    if (rc != MGF_OK) return rc;
+  }
   if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
   if (cg == 2) return dispatch<256, 2>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
   return dispatch<256, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);

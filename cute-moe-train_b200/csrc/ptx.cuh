@@ -172,6 +172,25 @@ __device__ __forceinline__ void umma_f8(uint32_t d_tmem, uint64_t a_desc, uint64
       : "memory");
 }
 
+// The same with a scale per row (A), column (B) and 32 elements of K, taken from TMEM (kind::mxf8f6f4, scales
+// UE8M0: the byte b stands for 2^(b - 127)); which byte of the scales' words is in the instruction descriptor.
+__device__ __forceinline__ void umma_mxf8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t sa_tmem, uint32_t sb_tmem, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(
+          d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sa_tmem), "r"(sb_tmem), "r"(accumulate)
+      : "memory");
+}
+
+// 32 rows of 16 bytes of shared memory to four TMEM columns, in each of the four 32-lane quarters; ordered
+// before the MMAs that this thread issues later.
+__device__ __forceinline__ void tmem_cp_32x128b_x4(uint32_t taddr, uint64_t smem_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(smem_desc) : "memory");
+}
+
 // Arrive on an mbarrier once all tcgen05 operations issued so far by this thread completed.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
@@ -312,6 +331,16 @@ __device__ __forceinline__ uint64_t make_smem_desc_sw128(uint32_t saddr, uint32_
   return d;
 }
 
+// Shared-memory descriptor of 8 x 16-byte core matrices without swizzle, `sbo_bytes` apart (scale factors).
+__device__ __forceinline__ uint64_t make_smem_desc_plain(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
+  d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
+  d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
+  d |= static_cast<uint64_t>(1u) << 46;
+  return d;
+}
+
 // Instruction descriptor for kind::f16 with bf16 A/B and fp32 accumulate.
 __host__ __device__ constexpr uint32_t make_idesc_bf16(int M, int N, bool a_mn_major, bool b_mn_major) {
   return (1u << 4)                                   // D format: f32
@@ -333,6 +362,20 @@ __host__ __device__ constexpr uint32_t make_idesc_e4m3(int M, int N, bool a_mn_m
          | ((b_mn_major ? 1u : 0u) << 16)            // B major
          | ((static_cast<uint32_t>(N) >> 3) << 17)   // N >> 3
          | ((static_cast<uint32_t>(M) >> 4) << 24);  // M >> 4
+}
+
+// Instruction descriptor for kind::mxf8f6f4 with e4m3 A and B, UE8M0 scales and fp32 accumulate; `sf` (0..3) is
+// the byte of the scale words that the instruction uses, for A and for B.
+__host__ __device__ constexpr uint32_t make_idesc_mxf8(int M, int N, bool a_mn_major, bool b_mn_major, uint32_t sf) {
+  return (sf << 4)                                   // B scale byte
+         | (0u << 7)                                 // A format: e4m3
+         | (0u << 10)                                // B format: e4m3
+         | ((a_mn_major ? 1u : 0u) << 15)            // A major
+         | ((b_mn_major ? 1u : 0u) << 16)            // B major
+         | ((static_cast<uint32_t>(N) >> 3) << 17)   // N >> 3
+         | (1u << 23)                                // scale format: UE8M0
+         | ((static_cast<uint32_t>(M) >> 7) << 27)   // M >> 7
+         | (sf << 29);                               // A scale byte
 }
 
 }  // namespace ptx

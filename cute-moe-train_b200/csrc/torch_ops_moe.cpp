@@ -362,6 +362,17 @@ BlockArgs block_args(const Tensor& a, const Tensor& b, const Tensor& offs, const
   return r;
 }
 
+// The launch with its scratch, which the caching allocator takes back in stream order.
+void launch_block(BlockArgs& r, const Tensor& a, const char* what) {
+  Tensor ws;
+  const int64_t bytes = mgf_block_gemm_workspace_bytes(&r.g);
+  if (bytes > 0) {
+    ws = at::empty({bytes}, a.options().dtype(at::kByte));
+    r.g.workspace = ws.data_ptr();
+  }
+  check_launch(mgf_block_gemm_launch(&r.g, stream()), what);
+}
+
 Tensor mm_fp8_block_cuda(const Tensor& a, const Tensor& b, const Tensor& offs, const Tensor& scale_a,
                          const Tensor& scale_b, const std::optional<Tensor>& bias) {
   BlockArgs r = block_args(a, b, offs, scale_a, scale_b, bias, "grouped_mm_fp8_block");
@@ -370,7 +381,7 @@ Tensor mm_fp8_block_cuda(const Tensor& a, const Tensor& b, const Tensor& offs, c
   r.g.epilogue = MGF_EPI_BIAS;
   r.g.d = out.data_ptr();
   r.g.ldd = out.stride(0);
-  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_fp8_block");
+  launch_block(r, a, "grouped_mm_fp8_block");
   return out;
 }
 
@@ -389,7 +400,7 @@ std::tuple<Tensor, Tensor> mm_swiglu_fp8_block_cuda(const Tensor& a, const Tenso
   r.g.ldd2 = s.stride(0);
   r.g.swiglu_alpha = static_cast<float>(alpha);
   r.g.swiglu_limit = static_cast<float>(limit);
-  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_swiglu_fp8_block");
+  launch_block(r, a, "grouped_mm_swiglu_fp8_block");
   return {s, aux};
 }
 
@@ -409,7 +420,7 @@ Tensor mm_swiglu_bwd_fp8_block_cuda(const Tensor& grad_output, const Tensor& dow
   r.g.ld_aux = stride_of(aux, 0, round_up(2 * r.n, 8));
   r.g.swiglu_alpha = static_cast<float>(alpha);
   r.g.swiglu_limit = static_cast<float>(limit);
-  check_launch(mgf_block_gemm_launch(&r.g, stream()), "grouped_mm_swiglu_bwd_fp8_block");
+  launch_block(r, grad_output, "grouped_mm_swiglu_bwd_fp8_block");
   return out;
 }
 

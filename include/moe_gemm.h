@@ -345,8 +345,14 @@ typedef struct mgf_block_gemm_desc {
   int64_t ld_aux;
   float swiglu_alpha;
   float swiglu_limit;
+  void* workspace;       /* device scratch of mgf_block_gemm_workspace_bytes(), 16-byte aligned, for this launch
+                            alone while it runs; NULL = the form that needs none */
 } mgf_block_gemm_desc;
 
+/* Two forms.  Where the workspace is given and every scale of a row in a group and of B turns out (on the device) to be
+ * a power of two in the normal range, the tensor cores apply the scales; otherwise every block's product is scaled
+ * and added in registers.  workspace_bytes: 0 where the first form would not pay. */
+int64_t mgf_block_gemm_workspace_bytes(const mgf_block_gemm_desc* desc);
 int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stream);
 size_t mgf_block_gemm_desc_size(void);
 

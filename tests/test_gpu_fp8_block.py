@@ -5,9 +5,11 @@ Tolerances of the products count roundings (u = 2^-24).  A block of 128 products
 by the tensor core: the products are exact (8 significant bits), the sum of 128 is allowed 128 roundings that
 may truncate instead of round (2 u each); the scale factor sa * sb rounds once, the promotion (one fused
 multiply-add per block) once per block.  So |acc - exact| <= (256 + 1 + blocks) u * S with S the sum of the
-magnitudes of all products.  bf16 output: 2^-8 of the value.  SwiGLU and its backward are computed from
+magnitudes of all products.  Where the tensor core applies the scales (powers of two: exact) it also sums all
+k products: 2 k u S.  bf16 output: 2^-8 of the value.  SwiGLU and its backward are computed from
 bf16 (exactly known) or fp32 inputs in fp32: a few u times their condition, below 64 u of the terms'
-magnitudes, times the output rounding.
+magnitudes, times the output rounding.  The sigmoid is 1 / (1 + e^-z) by the fast division, which gives 0 where
+the denominator is over 2^126: an absolute error of up to 2^-126, times the other factors.
 """
 
 from __future__ import annotations
@@ -244,21 +246,30 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("form", ["auto", "single", "pair", "narrow"])
+@pytest.mark.parametrize("form", ["auto", "single", "pair", "narrow", "choice", "powers"])
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 @pytest.mark.parametrize("E,K,N,counts", SHAPES)
 def test_products_against_64_bits(E, K, N, counts, layout, form, monkeypatch):
+    """auto .. narrow: the launch shapes; choice: arbitrary scales offered to the form that wants powers of two,
+    which has to leave them to the other; powers: powers of two, applied by the tensor cores."""
     import cutlass_op.bf16_grouped_mm as m
     from cutlass_op.bf16_grouped_mm import fp8_block
 
+    monkeypatch.setenv("MGF_BLOCK_MX", "1" if form in ("choice", "powers") else "0")
     if form in ("single", "pair"):
         monkeypatch.setenv("MGF_CTA_GROUP", "1" if form == "single" else "2")
     if form == "narrow":
         monkeypatch.setenv("MGF_BN", "128")
     a, b, offs, sa, sb, bias = _case(E, K, N, counts, layout, E * 7 + K, extra_rows=3)
     rows = int(offs[-1])
+    steps = 257 + sa.shape[1]
+    if form == "powers":
+        steps = 2 * K
+        for t in (sa, sb):
+            t.copy_(torch.exp2(torch.randint(-6, 7, t.shape, generator=_gen(8), device="cuda").float()))
+        sa[rows:] = 0.3  # behind the last group: no scale of the product
     acc, mag = _exact(a, b, offs, sa, sb)
-    tol = (257 + sa.shape[1]) * U * mag
+    tol = steps * U * mag
     out = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb)
     _within("no bias", out[:rows], acc[:rows], (tol + 2.0 ** -8 * acc.abs())[:rows])
     biased = acc + bias.double()[_row_of(offs, acc.shape[0])]
@@ -273,28 +284,29 @@ def test_products_against_64_bits(E, K, N, counts, layout, form, monkeypatch):
     biased = acc2 + bias2.double()[_row_of(offs, acc.shape[0])]
     s, aux = fp8_block.grouped_mm_swiglu_fp8_block(a, b, offs, sa2, sb, bias2, ALPHA, LIMIT)
     _within("aux", aux[:rows], biased[:rows],
-            ((257 + sa.shape[1]) * U * mag2 + U * biased.abs() + 2.0 ** -8 * biased.abs())[:rows])
+            (steps * U * mag2 + U * biased.abs() + 2.0 ** -8 * biased.abs())[:rows])
     gate, up = aux.double()[:, 0::2].clamp(max=LIMIT), aux.double()[:, 1::2].clamp(-LIMIT, LIMIT)
     ref = gate * torch.sigmoid(ALPHA * gate) * (up + 1)
     # exp of an argument of up to |alpha gate| with a rounding of its own: |z| u; u + 1 loses |up| u absolutely
     cond = (gate * torch.sigmoid(ALPHA * gate)).abs() * ((up + 1).abs() * (8 + 4 * (ALPHA * gate).abs()) + 2 * up.abs())
-    _within("swiglu", s[:rows], ref[:rows], (8 * U * cond + 2.0 ** -8 * ref.abs() + 1e-37)[:rows])
+    _within("swiglu", s[:rows], ref[:rows], (8 * U * cond + 2.0 ** -8 * ref.abs() + 2.0 ** -126 * (gate * (up + 1)).abs())[:rows])
     # SwiGLU backward against an aux with clamped and unclamped values
     aux_in = (4 * torch.randn(a.shape[0], 2 * N, generator=_gen(9), device="cuda")).to(torch.bfloat16)
     got = fp8_block.grouped_mm_swiglu_bwd_fp8_block(a, b, offs, aux_in, sa2, sb, ALPHA, LIMIT)
     g0, u0 = aux_in.double()[:, 0::2], aux_in.double()[:, 1::2]
     gc, uc = g0.clamp(max=LIMIT), u0.clamp(-LIMIT, LIMIT)
     sig = torch.sigmoid(ALPHA * gc)
-    err = (257 + sa.shape[1]) * U * mag2
+    err = steps * U * mag2
     fg = (uc + 1) * sig * (1 + ALPHA * gc * (1 - sig)) * (g0 <= LIMIT)
     fu = gc * sig * (u0.abs() <= LIMIT)
     z = (ALPHA * gc).abs()
     cg = sig * ((uc + 1).abs() * (1 + z) * (16 + 8 * z) + 2 * uc.abs() * (1 + z))
     cu = gc.abs() * sig * (8 + 4 * z)
+    tiny = 2.0 ** -126 * acc2.abs() * ((uc + 1).abs() + gc.abs()) * (1 + z)
     for name, f, c, part in (("d_gate", fg, cg, got[:, 0::2]), ("d_up", fu, cu, got[:, 1::2])):
         ref = acc2 * f
         _within(name, part[:rows], ref[:rows],
-                (err * (f.abs() + 8 * U * c) + 8 * U * c * acc2.abs() + 2.0 ** -8 * ref.abs() + 1e-37)[:rows])
+                (err * (f.abs() + 8 * U * c) + 8 * U * c * acc2.abs() + 2.0 ** -8 * ref.abs() + tiny + 1e-37)[:rows])
     m.check_device_status()
 
 
@@ -315,13 +327,13 @@ def test_rows_behind_the_last_group_stay_as_they_were():
                     ("sm_carveout", i32), ("offs", ptr), ("scale_a", ptr), ("scale_a_stride", i64), ("scale_b", ptr),
                     ("scale_b_stride_e", i64), ("scale_b_stride_k", i64), ("scale_b_stride_n", i64), ("bias", ptr),
                     ("bias_stride", i64), ("d", ptr), ("ldd", i64), ("d2", ptr), ("ldd2", i64), ("aux", ptr),
-                    ("ld_aux", i64), ("swiglu_alpha", f32), ("swiglu_limit", f32)]
+                    ("ld_aux", i64), ("swiglu_alpha", f32), ("swiglu_limit", f32), ("workspace", ptr)]
 
     _ext.lib.mgf_block_gemm_desc_size.restype = ctypes.c_size_t
     assert ctypes.sizeof(Desc) == _ext.lib.mgf_block_gemm_desc_size()
     d = Desc(0, 3, a.shape[0], 256, 256, a.data_ptr(), a.stride(0), b.data_ptr(), b.stride(1), b.stride(0), 1, 0,
              offs.data_ptr(), sa.data_ptr(), sa.stride(0), sb.data_ptr(), *sb.stride(), bias.data_ptr(), 256,
-             out.data_ptr(), 256, None, 0, None, 0, ALPHA, LIMIT)
+             out.data_ptr(), 256, None, 0, None, 0, ALPHA, LIMIT, None)
     _ext.lib.mgf_block_gemm_launch.argtypes = [ctypes.c_void_p, ctypes.c_void_p]
     assert _ext.lib.mgf_block_gemm_launch(ctypes.byref(d), torch.cuda.current_stream().cuda_stream) == 0
     assert torch.equal(out[:135], want[:135]) and (out[135:] == 7.0).all()
