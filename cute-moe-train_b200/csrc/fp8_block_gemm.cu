@@ -203,17 +203,26 @@ __device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, floa
   return pack_bf16x2(d_gate, d_up);
 }
 
-// Epilogue of one row's COLS columns from column c0 on.
-template <int EPI, int COLS>
-__device__ __forceinline__ void write_columns(const Params& p, const float (&acc)[COLS], int e, int grow, int c0) {
+// Epilogue of one row's COLS columns from column c0 on.  AHEAD (SWIGLU_BWD): aw holds the first 32 columns' aux words
+// and every chunk's are loaded one chunk ahead; otherwise they are loaded where they are used (fewer registers).
+template <int EPI, int COLS, bool AHEAD>
+__device__ __forceinline__ void write_columns(const Params& p, const float (&acc)[COLS], int e, int grow, int c0,
+                                              uint4 (&aw)[8]) {
   // 32 columns at a time; n is a multiple of 8 (SWIGLU: 16), so units of 8 columns are whole
 #pragma unroll
   for (int c = 0; c < COLS / 32; ++c) {
     const int col0 = c0 + c * 32;
     if (col0 >= p.n) break;
     if constexpr (EPI == MGF_EPI_SWIGLU_BWD) {
-      uint4 aw[8];
-      load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0, p.n, true, p.aux_v8, aw);
+      uint4 cur[8];
+      if constexpr (AHEAD) {
+#pragma unroll
+        for (int g = 0; g < 8; ++g) cur[g] = aw[g];
+        if (c + 1 < COLS / 32 && col0 + 32 < p.n)
+          load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0 + 32, p.n, true, p.aux_v8, aw);
+      } else {
+        load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, col0, p.n, true, p.aux_v8, cur);
+      }
       uint4* gp = reinterpret_cast<uint4*>(p.d + (int64_t)grow * p.ldd + 2 * col0);
       const int nvalid = (p.n - col0) >> 2;
 #pragma unroll
@@ -223,10 +232,10 @@ __device__ __forceinline__ void write_columns(const Params& p, const float (&acc
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float* f = acc + c * 32 + 4 * (g + h);
-            o[h].x = swiglu_bwd(f[0], aw[g + h].x, p.alpha, p.limit);
-            o[h].y = swiglu_bwd(f[1], aw[g + h].y, p.alpha, p.limit);
-            o[h].z = swiglu_bwd(f[2], aw[g + h].z, p.alpha, p.limit);
-            o[h].w = swiglu_bwd(f[3], aw[g + h].w, p.alpha, p.limit);
+            o[h].x = swiglu_bwd(f[0], cur[g + h].x, p.alpha, p.limit);
+            o[h].y = swiglu_bwd(f[1], cur[g + h].y, p.alpha, p.limit);
+            o[h].z = swiglu_bwd(f[2], cur[g + h].z, p.alpha, p.limit);
+            o[h].w = swiglu_bwd(f[3], cur[g + h].w, p.alpha, p.limit);
           }
           if (p.d_v8) ptx::st_v8(gp + g, o[0], o[1]);
           else {
@@ -485,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       if (!valid || !active) continue;
-      write_columns<EPI, COLS>(p, acc, ti.e, grow, c0);
+      uint4 aw[8];
+      write_columns<EPI, COLS, false>(p, acc, ti.e, grow, c0, aw);
     }
   }
 
@@ -561,6 +571,10 @@ struct MxCfg {
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + kSlots * SLOT_BYTES + BAR_BYTES + SCHED_BYTES;
   static constexpr int TMEM_COLS = 512, SFA_COL = BN, SFB_COL = BN + 4 * kSlots;
   static constexpr int kThreads = 384;  // producer, issuer, scales, schedule; 8 epilogue warps
+  // __launch_bounds__(384) gives the block 168 x 384 = 64512 registers; the first warpgroup hands back what it does
+  // not need: 72 x 128 + 216 x 256 = 64512.  The epilogue holds 128 accumulators and the aux words ahead.
+  static constexpr int kSetupRegs = 72, kEpiRegs = 216;
+  static_assert(kSetupRegs * 128 + kEpiRegs * 256 <= 168 * kThreads, "register split");
   static_assert(SMEM_BYTES <= 227 * 1024 && SFB_COL + 8 * kSlots <= TMEM_COLS, "shared and tensor memory");
 };
 
@@ -618,6 +632,8 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
   const int total_tiles = prefix[p.E];
   const int nk = (p.k + BK - 1) / BK, nkw = (nk + 3) / 4, nnb = (p.n + BK - 1) / BK;
 
+  if (warp < 4) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSetupRegs));
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
@@ -726,14 +742,19 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
         if (++slot == kSlots) { slot = 0; sphase ^= 1; }
       }
     }
-  } else if (warp >= 4) {
+  }
+  } else {
     // ------------------------------------------------------------ epilogue
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kEpiRegs));
     const int q = warp & 3, wg = (warp - 4) >> 2;
     uint32_t tphase = 0;
     for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, tphase ^= 1) {
       const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
       const int c0 = ti.n0 + wg * COLS, grow = ti.row0 + q * 32 + lane;
       const bool active = ti.row0 + q * 32 < ti.row_end && c0 < p.n;  // warp-uniform
+      uint4 aw[8];
+      if (EPI == MGF_EPI_SWIGLU_BWD && active && grow < ti.row_end)  // does not depend on the accumulator
+        load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, c0, p.n, true, p.aux_v8, aw);
       if (!__all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(tfull_bar), tphase, abort_flag, p.status))) break;
       ptx::tc_fence_after();
       float acc[COLS];
@@ -747,7 +768,7 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_relaxed(ptx::smem_u32(tempty_bar));
-      if (active && grow < ti.row_end) write_columns<EPI, COLS>(p, acc, ti.e, grow, c0);
+      if (active && grow < ti.row_end) write_columns<EPI, COLS, true>(p, acc, ti.e, grow, c0, aw);
     }
   }
 
