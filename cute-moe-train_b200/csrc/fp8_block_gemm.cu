@@ -54,8 +54,11 @@ struct Cfg {
   static constexpr int BUDGET = 227 * 1024 - 1024 - TAIL_BYTES;
   static constexpr int STAGES = BUDGET / STAGE_BYTES > 8 ? 8 : BUDGET / STAGE_BYTES;
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + TAIL_BYTES;
-  static constexpr int TMEM_COLS = 2 * BN;
-  static_assert(STAGES >= 3 && (2 * STAGES + 5) * 8 + 8 <= BAR_BYTES && SMEM_BYTES <= 227 * 1024, "shared memory");
+  // TMEM buffers: a buffer is away for about 1300 clocks around its products (commit, wake-up, drain, arrive,
+  // wake-up), which two buffers of 256 columns hide half of and four of 128 columns all of.
+  static constexpr int TMEM_COLS = 512;
+  static constexpr int BUFS = TMEM_COLS / BN;
+  static_assert(STAGES >= 3 && (2 * STAGES + 2 * BUFS + 1) * 8 + 8 <= BAR_BYTES && SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 
 struct Params {
@@ -279,8 +282,10 @@ __device__ __forceinline__ void write_columns(const Params& p, const float (&acc
 
 template <int BN, int EPI, bool B_MN, int CG>
 __global__ void __launch_bounds__(kThreads, 1)
-    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+    gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
+                const __grid_constant__ CUtensorMap tmB, const Params p) {
   using C = Cfg<BN, CG>;
+  constexpr int BUFS = C::BUFS;
   if (p.other_scales != nullptr && !any_other_scale(p)) return;
   constexpr int STAGES = C::STAGES;
   constexpr int TM = BM * CG;       // rows of a tile
@@ -294,9 +299,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full_bar = bars;
   uint64_t* empty_bar = bars + STAGES;
   uint64_t* tfull_bar = bars + 2 * STAGES;
-  uint64_t* tempty_bar = bars + 2 * STAGES + 2;
-  uint64_t* drain_bar = bars + 2 * STAGES + 4;
-  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  uint64_t* tempty_bar = bars + 2 * STAGES + BUFS;
+  uint64_t* drain_bar = bars + 2 * STAGES + 2 * BUFS;
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
   int* prefix = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES + C::BAR_BYTES);
   int* seg_start = prefix + (kMaxGroups + 1);
@@ -313,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(ptx::smem_u32(&full_bar[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
     }
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < BUFS; ++b) {
       ptx::mbar_init(ptx::smem_u32(&tfull_bar[b]), 1);
       ptx::mbar_init(ptx::smem_u32(&tempty_bar[b]), kNumEpiWarps * CG);
     }
@@ -356,6 +361,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
         const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
         const int nb0 = ti.n0 + static_cast<int>(crank) * C::BNC;
+        // a tile of up to 32 rows loads 32 rows of A; the products of the stage's other rows are never read
+        const bool few_rows = CG == 1 && ti.row_end - ti.row0 <= 32;
         for (int kb = 0; kb < nk; ++kb) {
           if (!wait_bounded(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status)) { ok = false; break; }
           uint32_t fb = ptx::smem_u32(&full_bar[stage]);
@@ -363,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (leader) ptx::mbar_arrive_expect_tx(fb, 2 * C::STAGE_BYTES);
             else fb = leader_addr(&full_bar[stage]);
           } else {
-            ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+            ptx::mbar_arrive_expect_tx(fb, few_rows ? 32 * BK + C::B_BYTES : C::STAGE_BYTES);
           }
           const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + C::A_BYTES;
           const int row = ti.row0 + static_cast<int>(crank) * BM;
@@ -372,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if constexpr (B_MN) ptx::tma_load_3d_pair(sB, &tmB, fb, nb0, kb * BK, ti.e);
             else ptx::tma_load_3d_pair(sB, &tmB, fb, kb * BK, nb0, ti.e);
           } else {
-            ptx::tma_load_2d(sA, &tmA, fb, kb * BK, row);
+            ptx::tma_load_2d(sA, few_rows ? &tmA32 : &tmA, fb, kb * BK, row);
             if constexpr (B_MN) {
 #pragma unroll
               for (int c = 0; c < C::BNC / 128; ++c)
@@ -401,12 +408,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
     constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
     constexpr uint32_t a_kstep = 32u >> 4;
-    uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, alternating TMEM buffers
+    uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, the TMEM buffers in turn
     bool ok = true, issued_any = false;
     if (leader && lane == 0) {
       for (int t = unit; ok && t < total_tiles; t += num_units) {
         for (int kb = 0; kb < nk; ++kb, ++part) {
-          const uint32_t buf = part & 1, bph = (part >> 1) & 1;
+          const uint32_t buf = part % BUFS, bph = (part / BUFS) & 1;
           ok = wait_bounded(ptx::smem_u32(&tempty_bar[buf]), bph ^ 1, abort_flag, p.status);
           if (!ok) break;
           ok = wait_bounded(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status);
@@ -446,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int q = warp & 3, wg = (warp - 2) >> 2;
     const int r = q * 32 + lane;
     const uint32_t lane_base = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + wg * COLS;
-    const uint32_t tempty_leader[2] = {leader_addr(&tempty_bar[0]), leader_addr(&tempty_bar[1])};
+    const uint32_t tempty_leader = leader_addr(tempty_bar);
     uint32_t part = 0;
     bool ok = true;
     for (int t = unit; ok && t < total_tiles; t += num_units) {
@@ -464,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float* sb_col = p.scale_b + ti.e * p.sb_e + (c0 / BK) * p.sb_n;
       float sa = active ? __ldg(sa_row) : 0.0f, sb = active ? __ldg(sb_col) : 0.0f;
       for (int kb = 0; kb < nk; ++kb, ++part) {
-        const uint32_t buf = part & 1, bph = (part >> 1) & 1;
+        const uint32_t buf = part % BUFS, bph = (part / BUFS) & 1;
         const float s = sa * sb;
         if (active && kb + 1 < nk) {
           sa = __ldg(sa_row + kb + 1);
@@ -488,7 +495,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ptx::tc_fence_before();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (CG == 2) arrive_relaxed_cluster(tempty_leader[buf]);
+          if constexpr (CG == 2) arrive_relaxed_cluster(tempty_leader + 8 * buf);
           else arrive_relaxed(ptx::smem_u32(&tempty_bar[buf]));
         }
       }
@@ -811,7 +818,8 @@ int launch_mx(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int
 }
 
 template <int BN, int EPI, bool B_MN, int CG>
-int launch(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
+int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+           cudaStream_t st) {
   auto kern = gemm_kernel<BN, EPI, B_MN, CG>;
   constexpr int smem = Cfg<BN, CG>::SMEM_BYTES;
   static std::mutex mu;
@@ -853,7 +861,7 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_
   if (tiles < units) units = static_cast<int>(tiles);
   cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
   cudaGetLastError();
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tA, tB, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tA, tA32, tB, p);
   if (e == cudaSuccess && debug_sync()) {
     e = cudaStreamSynchronize(st);
     fprintf(stderr, "[mgf] block-scaled BN=%d CG=%d epi=%d b_mn=%d units=%d E=%d rows=%lld n=%d k=%d -> %s\n", BN, CG,
@@ -867,18 +875,18 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_
 }
 
 template <int BN, int CG>
-int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
              cudaStream_t st) {
   switch (epi) {
     case MGF_EPI_BIAS:
-      return b_mn ? launch<BN, MGF_EPI_BIAS, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch<BN, MGF_EPI_BIAS, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch<BN, MGF_EPI_BIAS, true, CG>(tA, tA32, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_BIAS, false, CG>(tA, tA32, tB, p, tiles, sms, st);
     case MGF_EPI_SWIGLU:
-      return b_mn ? launch<BN, MGF_EPI_SWIGLU, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch<BN, MGF_EPI_SWIGLU, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch<BN, MGF_EPI_SWIGLU, true, CG>(tA, tA32, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_SWIGLU, false, CG>(tA, tA32, tB, p, tiles, sms, st);
     default:
-      return b_mn ? launch<BN, MGF_EPI_SWIGLU_BWD, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch<BN, MGF_EPI_SWIGLU_BWD, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch<BN, MGF_EPI_SWIGLU_BWD, true, CG>(tA, tA32, tB, p, tiles, sms, st)
+                  : launch<BN, MGF_EPI_SWIGLU_BWD, false, CG>(tA, tA32, tB, p, tiles, sms, st);
   }
 }
 
@@ -998,19 +1006,23 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   }
 
   // Pairs (256-row tiles, half the B bytes per SM) for groups of 512 rows and more on average, as in
-  // moe_gemm_sm100.cu; MGF_CTA_GROUP=1|2 forces.  128-column tiles only where one covers n.
+  // moe_gemm_sm100.cu; MGF_CTA_GROUP=1|2 forces.  128-column tiles where one covers n, and where 256-column tiles of
+  // the groups that can have rows would leave SMs without one (4 rows, n = 5760, k = 2880: 16.2 against 18.9 us);
+  // with more tiles the wide ones read fewer bytes of A per product (32 rows: 59.0 against 60.2 us, 256 rows: 97.5
+  // against 107).  MGF_BN=128|256 forces.
   const bool b_mn = g.b_mn_major != 0;
   int cg = g.total_rows / g.num_groups >= 512 ? 2 : 1;
   if (const char* env = getenv("MGF_CTA_GROUP"); env != nullptr && (env[0] == '1' || env[0] == '2')) cg = env[0] - '0';
-  int bn = g.n <= 128 ? 128 : 256;
+  const int64_t groups = g.total_rows < g.num_groups ? g.total_rows : g.num_groups;
+  int bn = g.n <= 128 || groups * ((g.n + 255) / 256) < di.sms ? 128 : 256;
   if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
   if (bn == 128) cg = 1;
   p.n_tiles = static_cast<int>((g.n + bn - 1) / bn);
 
-  CUtensorMap tA, tB;
+  CUtensorMap tA, tA32, tB;
   const uint64_t dA[2] = {static_cast<uint64_t>(g.k), static_cast<uint64_t>(g.total_rows)};
   const uint64_t sA[1] = {static_cast<uint64_t>(g.lda)};
-  const uint32_t bA[2] = {BK, BM};
+  const uint32_t bA[2] = {BK, BM}, bA32[2] = {BK, 32};
   const uint64_t batch = g.num_groups > 1 ? static_cast<uint64_t>(g.ldb_batch) : 16;
   const uint64_t sB[2] = {static_cast<uint64_t>(g.ldb), batch};
   const uint64_t dB_mn[3] = {static_cast<uint64_t>(g.n), static_cast<uint64_t>(g.k), static_cast<uint64_t>(g.num_groups)};
@@ -1019,6 +1031,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   const uint32_t bB_k[3] = {BK, static_cast<uint32_t>(bn / cg), 1};
   const auto u8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
   if (!encode_bf16(&tA, g.a, 2, dA, sA, bA, CU_TENSOR_MAP_SWIZZLE_128B, u8) ||
+      !encode_bf16(&tA32, g.a, 2, dA, sA, bA32, CU_TENSOR_MAP_SWIZZLE_128B, u8) ||
       !encode_bf16(&tB, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bB_k, CU_TENSOR_MAP_SWIZZLE_128B, u8))
     return MGF_ERR_CUDA;
 
@@ -1050,7 +1063,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
     const int rc = dispatch_mx(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st);
     if (rc != MGF_OK) return rc;
   }
-  if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
-  if (cg == 2) return dispatch<256, 2>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
-  return dispatch<256, 1>(g.epilogue, b_mn, tA, tB, p, tiles, sms, st);
+  if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);
+  if (cg == 2) return dispatch<256, 2>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);
+  return dispatch<256, 1>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);
 }
