@@ -41,17 +41,24 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float pow2_of(int biased) { return __uint_as_float(static_cast<uint32_t>(biased) << 23); }
 
-__device__ __forceinline__ float finite_abs(float v) {
-  const float a = fabsf(v);
-  return a <= 3.4028234663852886e38f ? a : 0.0f;  // NaN and infinity do not count
+// Magnitudes of bf16 pairs order like their bits without the sign, and those of NaN and infinity are the largest:
+// one packed maximum per pair finds amax and whether anything is not finite.  (Unpacking, comparing and testing
+// every element took 10 instructions each, as long as the memory traffic.)
+constexpr uint32_t kNotFinite = 0x7F80u;
+__device__ __forceinline__ uint32_t max_bits(uint32_t m, uint32_t pair) { return __vmaxu2(m, pair & 0x7FFF7FFFu); }
+__device__ __forceinline__ uint32_t larger_half(uint32_t m) { return max(m & 0xFFFFu, m >> 16); }
+// The same over finite elements only.
+__device__ __forceinline__ uint32_t max_finite_bits(uint32_t m, uint32_t pair) {
+  const uint32_t a = pair & 0x7FFFu, b = (pair >> 16) & 0x7FFFu;
+  return max(m, max(a < kNotFinite ? a : 0u, b < kNotFinite ? b : 0u));
 }
+__device__ __forceinline__ float of_bits(uint32_t bf16) { return __uint_as_float(bf16 << 16); }
 
-// Two codes: saturation never occurs for finite values (|x / s| <= 448); infinities become NaN like NaN.
+// Two codes.  Finite values never saturate (|x / s| <= 448); where the block holds others, they become NaN.
 __device__ __forceinline__ uint32_t code2(float a, float b, float inv) {
-  const float2 v = make_float2(isinf(a) ? __uint_as_float(0x7FC00000u) : a * inv,
-                               isinf(b) ? __uint_as_float(0x7FC00000u) : b * inv);
-  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3));
+  return static_cast<uint32_t>(__nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3));
 }
+__device__ __forceinline__ float no_infinity(float v) { return isinf(v) ? __uint_as_float(0x7FC00000u) : v; }
 
 __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
@@ -85,17 +92,34 @@ __global__ void __launch_bounds__(32 * kWarps)
         w[i] = l | (h << 16);
       }
     }
-    float amax = 0.0f;
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fmaxf(finite_abs(lo(w[i])), finite_abs(hi(w[i]))));
+    for (int i = 0; i < 8; ++i) m = max_bits(m, w[i]);
+    m = larger_half(m);
 #pragma unroll
-    for (int off = 4; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, off));
-    const int e = scale_exponent(amax);
+    for (int off = 4; off; off >>= 1) m = max(m, __shfl_xor_sync(kFull, m, off));
+    const bool all_finite = m < kNotFinite;
+    if (__any_sync(kFull, !all_finite)) {
+      uint32_t f = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f = max_finite_bits(f, w[i]);
+#pragma unroll
+      for (int off = 4; off; off >>= 1) f = max(f, __shfl_xor_sync(kFull, f, off));
+      m = f;
+    }
+    const int e = scale_exponent(of_bits(m));
     const float inv = pow2_of(254 - e);
     uint32_t c[4];
+    if (all_finite) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      c[i] = code2(lo(w[2 * i]), hi(w[2 * i]), inv) | (code2(lo(w[2 * i + 1]), hi(w[2 * i + 1]), inv) << 16);
+      for (int i = 0; i < 4; ++i)
+        c[i] = code2(lo(w[2 * i]), hi(w[2 * i]), inv) | (code2(lo(w[2 * i + 1]), hi(w[2 * i + 1]), inv) << 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        c[i] = code2(no_infinity(lo(w[2 * i])), no_infinity(hi(w[2 * i])), inv) |
+               (code2(no_infinity(lo(w[2 * i + 1])), no_infinity(hi(w[2 * i + 1])), inv) << 16);
+    }
     for (int j = 0; j < topk; ++j) {
       int64_t row = t;
       if (row_of_copy != nullptr) {
@@ -141,7 +165,7 @@ __global__ void __launch_bounds__(256)
     quantize_weights_kernel(const __nv_bfloat16* __restrict__ w, int64_t R, int64_t C, int64_t se, int64_t sr,
                             uint8_t* __restrict__ q, int64_t qe, int64_t qr, float* __restrict__ scale, int64_t ss_e,
                             int64_t ss_r, int64_t ss_c) {
-  __shared__ float red[8];
+  __shared__ uint32_t red[8];
   const int tid = threadIdx.x;
   const int64_t e = blockIdx.z, rb = blockIdx.y, cb = blockIdx.x;
   const int64_t r0 = rb * kBlock + (tid >> 4), c0 = cb * kBlock + (tid & 15) * 8;
@@ -162,28 +186,40 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
-  float amax = 0.0f;
+  // the block's largest magnitude; every thread takes part in every reduction
+  auto block_max = [&](uint32_t m) -> uint32_t {
+    m = __reduce_max_sync(kFull, m);
+    __syncthreads();  // the words of an earlier reduction have been read
+    if ((tid & 31) == 0) red[tid >> 5] = m;
+    __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t p[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    for (int i = 0; i < 8; ++i) m = max(m, red[i]);
+    return m;
+  };
+  uint32_t m = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) amax = fmaxf(amax, fmaxf(finite_abs(lo(p[k])), finite_abs(hi(p[k]))));
+  for (int i = 0; i < 8; ++i) m = max_bits(max_bits(max_bits(max_bits(m, v[i].x), v[i].y), v[i].z), v[i].w);
+  m = block_max(larger_half(m));
+  const bool all_finite = m < kNotFinite;  // the same for all threads
+  if (!all_finite) {
+    uint32_t f = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      f = max_finite_bits(max_finite_bits(max_finite_bits(max_finite_bits(f, v[i].x), v[i].y), v[i].z), v[i].w);
+    m = block_max(f);
   }
-#pragma unroll
-  for (int off = 16; off; off >>= 1) amax = fmaxf(amax, __shfl_xor_sync(kFull, amax, off));
-  if ((tid & 31) == 0) red[tid >> 5] = amax;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) amax = fmaxf(amax, red[i]);
-  const int ex = scale_exponent(amax);
+  const int ex = scale_exponent(of_bits(m));
   const float inv = pow2_of(254 - ex);
   if (tid == 0) scale[e * ss_e + rb * ss_r + cb * ss_c] = pow2_of(ex);
+  auto code4 = [&](uint32_t x, uint32_t y) -> uint32_t {
+    if (all_finite) return code2(lo(x), hi(x), inv) | (code2(lo(y), hi(y), inv) << 16);
+    return code2(no_infinity(lo(x)), no_infinity(hi(x)), inv) | (code2(no_infinity(lo(y)), no_infinity(hi(y)), inv) << 16);
+  };
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t r = r0 + 16 * i;
     if (r >= R) break;
-    const uint32_t c[2] = {code2(lo(v[i].x), hi(v[i].x), inv) | (code2(lo(v[i].y), hi(v[i].y), inv) << 16),
-                           code2(lo(v[i].z), hi(v[i].z), inv) | (code2(lo(v[i].w), hi(v[i].w), inv) << 16)};
+    const uint32_t c[2] = {code4(v[i].x, v[i].y), code4(v[i].z, v[i].w)};
     uint8_t* d = q + e * qe + r * qr + c0;
     if (c0 + 8 <= C) {
       *reinterpret_cast<uint2*>(d) = make_uint2(c[0], c[1]);

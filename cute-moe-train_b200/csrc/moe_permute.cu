@@ -499,6 +499,11 @@ extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_ex
   const unsigned threads = n <= 1024 ? least : 1024u;
   const unsigned ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
   const size_t smem = static_cast<size_t>(threads / 32 + 2) * num_experts * sizeof(int32_t);
+  if (ctas == 1) {
+    sort_kernel<<<1, threads, smem, static_cast<cudaStream_t>(stream)>>>(expert_idx, n, static_cast<int>(num_experts), offs,
+                                                                         row_of_copy, copy_of_row, status);
+    return launched();
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
