@@ -11,7 +11,6 @@
 // Everything but the sort moves rows once and is bound by HBM: 16-byte accesses, each token's row is read
 // once and written to its topk rows (not gathered once per row), several accesses in flight per thread.
 // No atomics: every sum has a fixed order, so results repeat bit for bit.
-#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -28,19 +27,19 @@ unsigned int* status_word_address();
 
 namespace {
 
-namespace cg = cooperative_groups;
-
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;  // warps per block of the row kernels
 
 // ---------------------------------------------------------------- sort
 constexpr int kSortBatch = 8;  // ids a lane loads together (and keeps from pass 1 to pass 2)
 
-// One cluster of CTAs sorts all copies in one launch.  The copies are split into contiguous ranges, one
-// per warp, and every warp keeps its own histogram in shared memory.  Pass 1 counts (shared-memory
-// atomics: a count has no order), the histograms are prefix-summed over the warps of a CTA, over the
-// CTAs (distributed shared memory) and over the experts, pass 2 walks the same ranges again 32 copies at a
-// time, ranks them within the warp and writes, so the order within an expert is the copies' order.
+// The copies are split into contiguous ranges, one per warp, and every warp keeps its own histogram in
+// shared memory.  Pass 1 counts (shared-memory atomics: a count has no order), the histograms are
+// prefix-summed over the warps of a CTA, over the CTAs and over the experts, pass 2 walks the same ranges
+// again 32 copies at a time, ranks them within the warp and writes, so the order within an expert is the
+// copies' order.  Up to 8192 copies one CTA does it all in one launch (3 us for 32 copies); above, a first
+// launch leaves every CTA's counts in the workspace.  (One launch of a cluster of 8 CTAs, counts exchanged in
+// distributed shared memory, took 17 us for 98304 copies: 8 SMs are too few for their scattered writes.)
 __device__ __forceinline__ void load_ids(const int64_t* ids, int64_t first, int64_t end, int E, int lane,
                                          int (&id)[kSortBatch], bool& bad) {
   int64_t v[kSortBatch];
@@ -68,25 +67,45 @@ __device__ __forceinline__ unsigned same_id(int id, int bits) {
   return same;
 }
 
-// blockDim.x: a multiple of 32, at least E, at most 1024.
+// Copies of CTA c of `ctas`: [c * per, (c + 1) * per).
+__device__ __host__ __forceinline__ int64_t copies_per_cta(int64_t n, int ctas) {
+  return ((n + ctas - 1) / ctas + 31) / 32 * 32;
+}
+
+// counts[cta][e] of every CTA's copies.
+__global__ void __launch_bounds__(256) count_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
+                                                    int32_t* __restrict__ counts) {
+  extern __shared__ int32_t smem[];
+  for (int e = threadIdx.x; e < E; e += blockDim.x) smem[e] = 0;
+  __syncthreads();
+  const int64_t per = copies_per_cta(n, gridDim.x), begin = blockIdx.x * per;
+  const int64_t end = begin + per < n ? begin + per : n;
+  for (int64_t i = begin + threadIdx.x; i < end; i += blockDim.x) {
+    const int64_t v = __ldg(ids + i);
+    if (v >= 0 && v < E) atomicAdd(smem + v, 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < E; e += blockDim.x) counts[static_cast<int64_t>(blockIdx.x) * E + e] = smem[e];
+}
+
+// blockDim.x: a multiple of 256, at least E, at most 1024.  counts: of all CTAs, nullptr for one CTA.
 __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
-                                                    int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
+                                                    const int32_t* __restrict__ counts, int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
                                                     int32_t* __restrict__ copy_of_row,
                                                     unsigned int* __restrict__ status) {
   extern __shared__ int32_t smem[];
   const int threads = blockDim.x, warps = threads >> 5;
   int32_t* hist = smem;                // [warps][E]
-  int32_t* total = smem + warps * E;   // [E] this CTA's counts, read by the other CTAs
+  int32_t* total = smem + warps * E;   // [E] this CTA's counts
   int32_t* base = total + E;           // [E] first row of this CTA's copies of each expert
   __shared__ int32_t warp_sums[32];
-  cg::cluster_group cluster = cg::this_cluster();
-  const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int ctas = gridDim.x, rank = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t units = static_cast<int64_t>(ctas) * warps;
-  const int64_t per = ((n + units - 1) / units + 31) / 32 * 32;
-  const int64_t unit = static_cast<int64_t>(rank) * warps + warp;
-  const int64_t begin = unit * per < n ? unit * per : n;
-  const int64_t end = begin + per < n ? begin + per : n;
+  const int64_t per_cta = copies_per_cta(n, ctas), per = ((per_cta + warps - 1) / warps + 31) / 32 * 32;
+  const int64_t first_copy = rank * per_cta < n ? rank * per_cta : n;
+  const int64_t last_copy = first_copy + per_cta < n ? first_copy + per_cta : n;
+  const int64_t begin = first_copy + warp * per < last_copy ? first_copy + warp * per : last_copy;
+  const int64_t end = begin + per < last_copy ? begin + per : last_copy;
   const int bits = 32 - __clz(E);  // of the largest id + 1
   bool bad = false;
   int id[kSortBatch];
@@ -120,16 +139,20 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ 
     }
     total[e] = run;
   }
-  if (ctas > 1) cluster.sync();
-  else __syncthreads();
+  __syncthreads();
   // one expert per thread: counts of all CTAs and of those before this one
   int32_t all = 0, before = 0;
   if (threadIdx.x < E) {
-    if (ctas > 1) {
-      for (int c = 0; c < ctas; ++c) {
-        const int32_t v = cluster.map_shared_rank(total, c)[threadIdx.x];
-        all += v;
-        before += c < rank ? v : 0;
+    if (counts != nullptr) {
+      for (int c0 = 0; c0 < ctas; c0 += 16) {
+        int32_t v[16];
+#pragma unroll
+        for (int c = 0; c < 16; ++c) v[c] = c0 + c < ctas ? __ldg(counts + static_cast<int64_t>(c0 + c) * E + threadIdx.x) : 0;
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          all += v[c];
+          before += c0 + c < rank ? v[c] : 0;
+        }
       }
     } else {
       all = total[threadIdx.x];
@@ -183,7 +206,6 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ 
   for (int64_t r = kept + static_cast<int64_t>(rank) * threads + threadIdx.x; r < n;
        r += static_cast<int64_t>(ctas) * threads)
     copy_of_row[r] = -1;
-  if (ctas > 1) cluster.sync();  // no CTA leaves while another may still read its counts
 }
 
 // ---------------------------------------------------------------- row access
@@ -475,13 +497,27 @@ bool grid_of(int64_t units, unsigned& grid) {
 }  // namespace
 }  // namespace mgf
 
+// CTAs of a sort in two launches: 2048 copies each up to one wave of them.
+static int sort_ctas(int64_t n) {
+  if (n <= 8192) return 1;
+  const int64_t c = (n + 2047) / 2048;
+  return static_cast<int>(c < 148 ? c : 148);
+}
+
+extern "C" int64_t mgf_moe_sort_workspace_words(int64_t n, int32_t num_experts) {
+  const int ctas = sort_ctas(n);
+  return ctas > 1 ? static_cast<int64_t>(ctas) * num_experts : 0;
+}
+
 extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int32_t* offs,
-                            int32_t* row_of_copy, int32_t* copy_of_row, void* stream) {
+                            int32_t* row_of_copy, int32_t* copy_of_row, int32_t* workspace, void* stream) {
   using namespace mgf;
   if (n < 0 || n > INT32_MAX || num_experts < 1 || num_experts > 1024 || offs == nullptr)
     return MGF_ERR_INVALID_ARGUMENT;
   if (n > 0 && (expert_idx == nullptr || row_of_copy == nullptr || copy_of_row == nullptr))
     return MGF_ERR_INVALID_ARGUMENT;
+  const int ctas = sort_ctas(n);
+  if (ctas > 1 && workspace == nullptr) return MGF_ERR_INVALID_ARGUMENT;
   unsigned int* status = status_word_address();
   if (status == nullptr) return MGF_ERR_CUDA;
   int dev = 0;
@@ -493,33 +529,18 @@ extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_ex
       return MGF_ERR_CUDA;
     attr_done[dev] = true;
   }
-  // few copies: 8 warps (as many as E needs threads); then one CTA of 32 warps up to 128 copies per warp, then
-  // 2, 4 and 8 CTAs (the portable cluster size)
-  const unsigned least = (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
-  const unsigned threads = n <= 1024 ? least : 1024u;
-  const unsigned ctas = n <= 4096 ? 1 : n <= 8192 ? 2 : n <= 16384 ? 4 : 8;
-  const size_t smem = static_cast<size_t>(threads / 32 + 2) * num_experts * sizeof(int32_t);
-  if (ctas == 1) {
-    sort_kernel<<<1, threads, smem, static_cast<cudaStream_t>(stream)>>>(expert_idx, n, static_cast<int>(num_experts), offs,
-                                                                         row_of_copy, copy_of_row, status);
-    return launched();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (ctas > 1) {
+    count_kernel<<<ctas, 256, num_experts * sizeof(int32_t), st>>>(expert_idx, n, num_experts, workspace);
+    if (launched() != MGF_OK) return MGF_ERR_CUDA;
   }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sort_kernel, expert_idx, n, static_cast<int>(num_experts), offs, row_of_copy,
-                            copy_of_row, status) == cudaSuccess
-             ? MGF_OK
-             : MGF_ERR_CUDA;
+  // 8 warps, or as many as E needs threads; all 32 where one CTA has many copies
+  const unsigned least = (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
+  const unsigned threads = ctas == 1 && n > 1024 ? 1024u : least;
+  const size_t smem = static_cast<size_t>(threads / 32 + 2) * num_experts * sizeof(int32_t);
+  sort_kernel<<<ctas, threads, smem, st>>>(expert_idx, n, num_experts, ctas > 1 ? workspace : nullptr, offs, row_of_copy,
+                                           copy_of_row, status);
+  return launched();
 }
 
 extern "C" int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden,

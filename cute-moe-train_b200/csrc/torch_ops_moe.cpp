@@ -126,9 +126,12 @@ std::tuple<Tensor, Tensor, Tensor> moe_sort_cuda(const Tensor& expert_idx, int64
   const c10::cuda::CUDAGuard guard(expert_idx.device());
   const auto o = expert_idx.options().dtype(at::kInt);
   Tensor offs = at::empty({num_experts}, o), row_of_copy = at::empty(expert_idx.sizes(), o), copy_of_row = at::empty({n}, o);
+  Tensor ws;
+  const int64_t words = mgf_moe_sort_workspace_words(n, static_cast<int32_t>(num_experts));
+  if (words > 0) ws = at::empty({words}, o);
   check_launch(mgf_moe_sort(expert_idx.data_ptr<int64_t>(), n, static_cast<int32_t>(num_experts),
                             offs.data_ptr<int32_t>(), row_of_copy.data_ptr<int32_t>(), copy_of_row.data_ptr<int32_t>(),
-                            stream()),
+                            words > 0 ? ws.data_ptr<int32_t>() : nullptr, stream()),
                "moe_sort");
   return {offs, row_of_copy, copy_of_row};
 }

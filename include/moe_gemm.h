@@ -272,9 +272,11 @@ int mgf_moe_route_bwd(const void* logits, int32_t dtype, int64_t ld, int64_t tok
 /* Plan of the permutation: stable counting sort of n routed copies (expert_idx int64 [n], copy c = token
  * c / topk) by expert, E <= 1024.  offs int32 [E] (cumulative row ends, what the grouped products take),
  * row_of_copy int32 [n] (-1 for a copy whose id is -1), copy_of_row int32 [n] (-1 behind offs[E-1]).  Ids
- * outside [-1, E) drop their copy too and set MGF_DEV_ROW_OUT_OF_RANGE.  One launch. */
+ * outside [-1, E) drop their copy too and set MGF_DEV_ROW_OUT_OF_RANGE.  workspace: int32
+ * [mgf_moe_sort_workspace_words(n, E)] device scratch of this call (may be NULL where that is 0). */
+int64_t mgf_moe_sort_workspace_words(int64_t n, int32_t num_experts);
 int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int32_t* offs, int32_t* row_of_copy,
-                 int32_t* copy_of_row, void* stream);
+                 int32_t* copy_of_row, int32_t* workspace, void* stream);
 
 /* Rows by a plan (any hidden size; strides in elements; 16-byte accesses where every base and pitch and the
  * width allow).  offs_end points at offs[E-1].  A row index >= n_rows is skipped and sets

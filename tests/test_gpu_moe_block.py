@@ -227,8 +227,8 @@ def test_sort_equals_a_stable_counting_sort(T, k, E, drop):
     _status_ok()
 
 
-@pytest.mark.parametrize("n,E", [(4096 * 2 + 5, 16), (4096 * 4 + 1, 1024), (300_001, 128)])
-def test_sort_of_many_copies_on_every_cluster_size(n, E):
+@pytest.mark.parametrize("n,E", [(8192, 64), (8193, 16), (4096 * 4 + 1, 1024), (300_001, 128), (700_000, 3)])
+def test_sort_of_many_copies(n, E):
     from cutlass_op.bf16_grouped_mm.permute import moe_sort
 
     idx = _ids(_gen(n), n, 1, E, 0.05)

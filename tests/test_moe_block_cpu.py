@@ -75,9 +75,13 @@ def test_host_refusals_at_the_c_abi():
     assert r(logits=None) == -1 and r() == -1  # outputs missing
     assert r(tokens=0) == 0
     sort = lib.mgf_moe_sort
-    sort.argtypes = [ptr, i64, i32, ptr, ptr, ptr, ptr]
-    assert sort(None, 4, 8, 16, 16, 16, None) == -1 and sort(16, -1, 8, 16, 16, 16, None) == -1
-    assert sort(16, 1 << 31, 8, 16, 16, 16, None) == -1 and sort(16, 4, 1025, 16, 16, 16, None) == -1
+    sort.argtypes = [ptr, i64, i32, ptr, ptr, ptr, ptr, ptr]
+    assert sort(None, 4, 8, 16, 16, 16, None, None) == -1 and sort(16, -1, 8, 16, 16, 16, None, None) == -1
+    assert sort(16, 1 << 31, 8, 16, 16, 16, 16, None) == -1 and sort(16, 4, 1025, 16, 16, 16, None, None) == -1
+    assert sort(16, 9000, 8, 16, 16, 16, None, None) == -1  # needs its workspace
+    lib.mgf_moe_sort_workspace_words.restype = i64
+    lib.mgf_moe_sort_workspace_words.argtypes = [i64, i32]
+    assert lib.mgf_moe_sort_workspace_words(8192, 8) == 0 and lib.mgf_moe_sort_workspace_words(8193, 8) == 40
     quant = lib.mgf_fp8_block_quantize_rows
     quant.argtypes = [ptr, i64, i64, i64, i32, ptr, ptr, ptr, i64, ptr, i64, i64, ptr]
     assert quant(16, 8, 4, 8, 2, None, None, 16, 16, 16, 4, 4, None) == -1   # two rows per token without a plan
