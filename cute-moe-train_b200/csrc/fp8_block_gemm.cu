@@ -134,6 +134,15 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
   return true;
 }
 
+// The same for the barrier that the scales of both CTAs of a pair arrive on: acquired at cluster scope.
+template <int CG>
+__device__ __forceinline__ bool wait_scales_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
+                                                    unsigned int* status) {
+  if constexpr (CG == 1) return wait_bounded(bar, parity, abort_flag, status);
+  if (!wait_bounded(bar, parity, abort_flag, status)) return false;
+  return ptx::mbar_try_wait_cluster(bar, parity);  // the phase is complete: this only acquires
+}
+
 // Group bounds clamped into [0, total_rows] and the prefix of their tile counts; one warp.
 template <int TM>
 __device__ void build_schedule(const Params& p, int* prefix, int* seg_start, int* seg_end, int lane) {
@@ -567,10 +576,12 @@ __global__ void __launch_bounds__(256) pack_scales_kernel(const Params p, uint32
 // TMEM: the accumulator's 256 columns, then kSlots scale slots of 4 columns (A: one word per row of 32 x 4) and of 8
 // (B: one word per column of 32 x 8).  One accumulator: the epilogue takes it into registers and hands it back before
 // it converts and stores, so that the next tile's products run under the stores.
+template <int CG>
 struct MxCfg {
   static constexpr int BN = 256;
-  static constexpr int STAGE_BYTES = BM * BK + BN * BK;
-  static constexpr int STAGES = 4;
+  static constexpr int BNC = BN / CG;  // columns of B held by this CTA
+  static constexpr int STAGE_BYTES = BM * BK + BNC * BK;
+  static constexpr int STAGES = CG == 2 ? 6 : 4;
   static constexpr int kSlots = 4;               // each holds the scales of four blocks of k
   static constexpr int SLOT_BYTES = 512 + 1024;  // 128 rows of A, 256 columns of B
   static constexpr int BAR_BYTES = 512;
@@ -585,10 +596,13 @@ struct MxCfg {
   static_assert(SMEM_BYTES <= 227 * 1024 && SFB_COL + 8 * kSlots <= TMEM_COLS, "shared and tensor memory");
 };
 
-template <int EPI, bool B_MN>
-__global__ void __launch_bounds__(MxCfg::kThreads, 1)
+// CG = 2: a pair of CTAs on a 256 x 256 tile; each loads its 128 rows of A and 128 columns of B and holds the scales of its
+// rows and of all columns, the even CTA issues.
+template <int EPI, bool B_MN, int CG>
+__global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
     mx_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
-  using C = MxCfg;
+  using C = MxCfg<CG>;
+  constexpr int TM = BM * CG;
   constexpr int STAGES = C::STAGES, BN = C::BN, COLS = BN / 2, kSlots = C::kSlots;
   if (any_other_scale(p)) return;
 
@@ -609,6 +623,19 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
   int* seg_start = prefix + (kMaxGroups + 1);
   int* seg_end = seg_start + (kMaxGroups + 1);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t crank = CG == 2 ? ptx::cluster_ctarank() : 0u;
+  const bool leader = crank == 0;
+  const int unit = CG == 2 ? static_cast<int>(blockIdx.x >> 1) : static_cast<int>(blockIdx.x);
+  const int num_units = CG == 2 ? static_cast<int>(gridDim.x >> 1) : static_cast<int>(gridDim.x);
+  auto leader_addr = [&](const void* ptr) -> uint32_t {
+    const uint32_t a = ptx::smem_u32(ptr);
+    if constexpr (CG == 2) return ptx::mapa_shared(a, 0);
+    return a;
+  };
+  auto commit = [&](const void* bar) {  // on this CTA's barrier, or the same one of both CTAs of a pair
+    if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(bar), 0x3);
+    else ptx::umma_commit(ptx::smem_u32(bar));
+  };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -616,11 +643,11 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
       ptx::mbar_init(ptx::smem_u32(&empty_bar[s]), 1);
     }
     for (int s = 0; s < kSlots; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&sf_full[s]), 32);
+      ptx::mbar_init(ptx::smem_u32(&sf_full[s]), CG);
       ptx::mbar_init(ptx::smem_u32(&sf_empty[s]), 1);
     }
     ptx::mbar_init(ptx::smem_u32(tfull_bar), 1);
-    ptx::mbar_init(ptx::smem_u32(tempty_bar), kNumEpiWarps);
+    ptx::mbar_init(ptx::smem_u32(tempty_bar), kNumEpiWarps * CG);
     ptx::mbar_init(ptx::smem_u32(drain_bar), 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -628,12 +655,18 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
     ptx::prefetch_tmap(&tmB);
   }
   if (warp == 1) {
-    ptx::tmem_alloc(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
-    ptx::tmem_relinquish();
+    if constexpr (CG == 2) {
+      ptx::tmem_alloc_pair(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
+      ptx::tmem_relinquish_pair();
+    } else {
+      ptx::tmem_alloc(ptx::smem_u32(tmem_holder), C::TMEM_COLS);
+      ptx::tmem_relinquish();
+    }
   }
-  if (warp == 3) build_schedule<BM>(p, prefix, seg_start, seg_end, lane);
+  if (warp == 3) build_schedule<TM>(p, prefix, seg_start, seg_end, lane);
   ptx::tc_fence_before();
   __syncthreads();
+  if constexpr (CG == 2) ptx::cluster_sync();  // barriers of both CTAs initialised before any remote use
   ptx::tc_fence_after();
   const uint32_t tmem_base = *tmem_holder;
   const int total_tiles = prefix[p.E];
@@ -647,54 +680,70 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
       uint32_t stage = 0, phase = 0;
       uint32_t issued = 0, issued_parity = 0;  // one bit per stage
       bool ok = true;
-      for (int t = blockIdx.x; ok && t < total_tiles && !p.stall_test; t += gridDim.x) {
-        const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
+      for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+        const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
         for (int kb = 0; kb < nk; ++kb) {
           if (!wait_bounded(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status)) { ok = false; break; }
-          const uint32_t fb = ptx::smem_u32(&full_bar[stage]);
-          ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
-          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + BM * BK;
-          ptx::tma_load_2d(sA, &tmA, fb, kb * BK, ti.row0);
-          if constexpr (B_MN) {
-            ptx::tma_load_3d(sB, &tmB, fb, ti.n0, kb * BK, ti.e);
-            ptx::tma_load_3d(sB + 16384, &tmB, fb, ti.n0 + 128, kb * BK, ti.e);
+          uint32_t fb = ptx::smem_u32(&full_bar[stage]);
+          if constexpr (CG == 2) {  // both CTAs' bytes count on the even CTA's barrier
+            if (leader) ptx::mbar_arrive_expect_tx(fb, 2 * C::STAGE_BYTES);
+            else fb = leader_addr(&full_bar[stage]);
           } else {
-            ptx::tma_load_3d(sB, &tmB, fb, kb * BK, ti.n0, ti.e);
+            ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+          }
+          const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + BM * BK;
+          const int row = ti.row0 + static_cast<int>(crank) * BM, col = ti.n0 + static_cast<int>(crank) * C::BNC;
+          if constexpr (CG == 2) {
+            ptx::tma_load_2d_pair(sA, &tmA, fb, kb * BK, row);
+            if constexpr (B_MN) ptx::tma_load_3d_pair(sB, &tmB, fb, col, kb * BK, ti.e);
+            else ptx::tma_load_3d_pair(sB, &tmB, fb, kb * BK, col, ti.e);
+          } else {
+            ptx::tma_load_2d(sA, &tmA, fb, kb * BK, row);
+            if constexpr (B_MN) {
+              ptx::tma_load_3d(sB, &tmB, fb, col, kb * BK, ti.e);
+              ptx::tma_load_3d(sB + 16384, &tmB, fb, col + 128, kb * BK, ti.e);
+            } else {
+              ptx::tma_load_3d(sB, &tmB, fb, kb * BK, col, ti.e);
+            }
           }
           issued |= 1u << stage;
           issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok) {  // stopped early: let the copies in flight land before the CTA exits
+      if (!ok && CG == 1) {  // stopped early: let the copies in flight land before the CTA exits (a pair meets below)
         for (int s = 0; s < STAGES; ++s)
           if ((issued >> s) & 1u)
             wait_bounded(ptx::smem_u32(&full_bar[s]), (issued_parity >> s) & 1u, abort_flag, p.status, kDrainLimitNs);
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ UMMA issuer (one thread)
-    if (lane == 0) {
+    // ------------------------------------------------------------ UMMA issuer (one thread of the even CTA)
+    if (leader && lane == 0) {
       constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
       constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
       constexpr uint32_t a_kstep = 32u >> 4;
       uint32_t stage = 0, phase = 0, slot = 0, sphase = 0, tphase = 0;
       bool ok = true, issued_any = false;
-      for (int t = blockIdx.x; ok && t < total_tiles; t += gridDim.x, tphase ^= 1) {
+      for (int t = unit; ok && t < total_tiles; t += num_units, tphase ^= 1) {
         ok = wait_bounded(ptx::smem_u32(tempty_bar), tphase ^ 1, abort_flag, p.status);
         if (!ok) break;
         ptx::tc_fence_after();
         uint32_t sfa = 0, sfb = 0;
         for (int kb = 0; kb < nk; ++kb) {
           if ((kb & 3) == 0) {  // the scales of the next four blocks
-            ok = wait_bounded(ptx::smem_u32(&sf_full[slot]), sphase, abort_flag, p.status);
+            ok = wait_scales_bounded<CG>(ptx::smem_u32(&sf_full[slot]), sphase, abort_flag, p.status);
             if (!ok) break;
             const uint32_t src = ptx::smem_u32(slots + slot * C::SLOT_BYTES);
             sfa = tmem_base + C::SFA_COL + 4 * slot;
             sfb = tmem_base + C::SFB_COL + 8 * slot;
-            ptx::tmem_cp_32x128b_x4(sfa, ptx::make_smem_desc_plain(src, 16, 128));
-            ptx::tmem_cp_32x128b_x4(sfb, ptx::make_smem_desc_plain(src + 512, 16, 128));
-            ptx::tmem_cp_32x128b_x4(sfb + 4, ptx::make_smem_desc_plain(src + 1024, 16, 128));
+#pragma unroll
+            for (int j = 0; j < 3; ++j) {  // 128 rows of A, 2 x 128 columns of B
+              const uint32_t dst = j == 0 ? sfa : sfb + 4 * (j - 1);
+              const uint64_t desc = ptx::make_smem_desc_plain(src + 512 * j, 16, 128);
+              if constexpr (CG == 2) ptx::tmem_cp_32x128b_x4_pair(dst, desc);
+              else ptx::tmem_cp_32x128b_x4(dst, desc);
+            }
           }
           ok = wait_bounded(ptx::smem_u32(&full_bar[stage]), phase, abort_flag, p.status);
           if (!ok) break;
@@ -702,23 +751,28 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
           const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES);
           const uint64_t adesc = ptx::make_smem_desc_sw128(sA, 16, 1024);
           const uint64_t bdesc = ptx::make_smem_desc_sw128(sA + BM * BK, b_lbo, 1024);
-          const uint32_t idesc = ptx::make_idesc_mxf8(BM, BN, false, B_MN, kb & 3);
+          const uint32_t idesc = ptx::make_idesc_mxf8(TM, BN, false, B_MN, kb & 3);
 #pragma unroll
-          for (int kk = 0; kk < BK / 32; ++kk)
-            ptx::umma_mxf8(tmem_base, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, sfa, sfb, (kb | kk) != 0);
+          for (int kk = 0; kk < BK / 32; ++kk) {
+            if constexpr (CG == 2)
+              ptx::umma_mxf8_pair(tmem_base, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, sfa, sfb, (kb | kk) != 0);
+            else
+              ptx::umma_mxf8(tmem_base, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, sfa, sfb, (kb | kk) != 0);
+          }
           issued_any = true;
-          ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
+          commit(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
           if ((kb & 3) == 3 || kb == nk - 1) {
-            ptx::umma_commit(ptx::smem_u32(&sf_empty[slot]));
+            commit(&sf_empty[slot]);
             if (++slot == kSlots) { slot = 0; sphase ^= 1; }
           }
         }
         if (!ok) break;
-        ptx::umma_commit(ptx::smem_u32(tfull_bar));
+        commit(tfull_bar);
       }
       if (!ok && issued_any) {  // stopped early: wait for the UMMAs already issued before TMEM is released
-        ptx::umma_commit(ptx::smem_u32(drain_bar));
+        if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
+        else ptx::umma_commit(ptx::smem_u32(drain_bar));
         wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, p.status, kDrainLimitNs);
       }
     }
@@ -729,9 +783,9 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
     // columns for B, which within one block of 128 are all the same word).
     uint32_t slot = 0, sphase = 0;
     bool ok = true;
-    for (int t = blockIdx.x; ok && t < total_tiles && !p.stall_test; t += gridDim.x) {
-      const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
-      const uint32_t* pa = p.packed_a + ti.row0 + lane;
+    for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+      const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
+      const uint32_t* pa = p.packed_a + ti.row0 + static_cast<int>(crank) * BM + lane;
       const int c0 = ti.n0 / BK, c1 = c0 + 1 < nnb ? c0 + 1 : c0;
       const uint32_t* pb = p.packed_b + static_cast<int64_t>(ti.e) * nkw * nnb;
       for (int w = 0; w < nkw; ++w) {
@@ -745,7 +799,11 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
         dst[32] = make_uint4(b0, b0, b0, b0);
         dst[64] = make_uint4(b1, b1, b1, b1);
         ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(ptx::smem_u32(&sf_full[slot]));
+        __syncwarp();
+        if (lane == 0) {  // the even CTA issues the copies of both
+          if constexpr (CG == 2) ptx::mbar_arrive_cluster(leader_addr(&sf_full[slot]));
+          else ptx::mbar_arrive(ptx::smem_u32(&sf_full[slot]));
+        }
         if (++slot == kSlots) { slot = 0; sphase ^= 1; }
       }
     }
@@ -755,10 +813,11 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kEpiRegs));
     const int q = warp & 3, wg = (warp - 4) >> 2;
     uint32_t tphase = 0;
-    for (int t = blockIdx.x; t < total_tiles; t += gridDim.x, tphase ^= 1) {
-      const Tile ti = decode_tile<BM, BN>(t, p, prefix, seg_start, seg_end);
-      const int c0 = ti.n0 + wg * COLS, grow = ti.row0 + q * 32 + lane;
-      const bool active = ti.row0 + q * 32 < ti.row_end && c0 < p.n;  // warp-uniform
+    for (int t = unit; t < total_tiles; t += num_units, tphase ^= 1) {
+      const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
+      const int crow0 = ti.row0 + static_cast<int>(crank) * BM;  // first row of this CTA's half
+      const int c0 = ti.n0 + wg * COLS, grow = crow0 + q * 32 + lane;
+      const bool active = crow0 + q * 32 < ti.row_end && c0 < p.n;  // warp-uniform
       uint4 aw[8];
       if (EPI == MGF_EPI_SWIGLU_BWD && active && grow < ti.row_end)  // does not depend on the accumulator
         load_aux_chunk(p.aux + (int64_t)grow * p.ld_aux, c0, p.n, true, p.aux_v8, aw);
@@ -774,54 +833,30 @@ __global__ void __launch_bounds__(MxCfg::kThreads, 1)
       }
       ptx::tc_fence_before();
       __syncwarp();
-      if (lane == 0) arrive_relaxed(ptx::smem_u32(tempty_bar));
+      if (lane == 0) {
+        if constexpr (CG == 2) arrive_relaxed_cluster(leader_addr(tempty_bar));
+        else arrive_relaxed(ptx::smem_u32(tempty_bar));
+      }
       if (active && grow < ti.row_end) write_columns<EPI, COLS, true>(p, acc, ti.e, grow, c0, aw);
     }
   }
 
   ptx::tc_fence_before();
   __syncthreads();
+  // A pair leaves together: the peer may still signal this CTA's barriers until both are done.
+  if constexpr (CG == 2) ptx::cluster_sync();
   if (warp == 1) {
     ptx::tc_fence_after();
-    ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
+    if constexpr (CG == 2) ptx::tmem_dealloc_pair(tmem_base, C::TMEM_COLS);
+    else ptx::tmem_dealloc(tmem_base, C::TMEM_COLS);
   }
 }
 
-template <int EPI, bool B_MN>
-int launch_mx(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
-  auto kern = mx_kernel<EPI, B_MN>;
-  static std::atomic<bool> attr_done[64];
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return MGF_ERR_CUDA;
-  if (!attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MxCfg::SMEM_BYTES);
-    if (e != cudaSuccess) {
-      record_error("cudaFuncSetAttribute", e);
-      return MGF_ERR_CUDA;
-    }
-    attr_done[dev] = true;
-  }
-  const unsigned grid = static_cast<unsigned>(tiles < sms ? tiles : sms);
-  cudaGetLastError();
-  kern<<<grid, MxCfg::kThreads, MxCfg::SMEM_BYTES, st>>>(tA, tB, p);
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess && debug_sync()) {
-    e = cudaStreamSynchronize(st);
-    fprintf(stderr, "[mgf] block-scaled mx epi=%d b_mn=%d grid=%u E=%d rows=%lld n=%d k=%d -> %s\n", EPI, int(B_MN), grid,
-            p.E, (long long)p.total_rows, p.n, p.k, cudaGetErrorString(e));
-  }
-  if (e != cudaSuccess) {
-    record_error("kernel launch", e);
-    return MGF_ERR_CUDA;
-  }
-  return MGF_OK;
-}
-
-template <int BN, int EPI, bool B_MN, int CG>
-int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
-           cudaStream_t st) {
-  auto kern = gemm_kernel<BN, EPI, B_MN, CG>;
-  constexpr int smem = Cfg<BN, CG>::SMEM_BYTES;
+// Launch of a persistent kernel with at most one CTA (or pair of CTAs) per SM (or pair of SMs).  A template on the
+// kernel itself: what it remembers per device belongs to that kernel.
+template <auto KERN, int CG, typename... Args>
+int launch_persistent(int threads, int smem, const char* form, int epi, bool b_mn, const Params& p, int64_t tiles, int sms,
+                      cudaStream_t st, const Args&... args) {
   static std::mutex mu;
   static bool attr_done[64] = {};
   static int max_units[64] = {};
@@ -831,8 +866,8 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = static_cast<size_t>(smem);
   cfg.stream = st;
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = CG;
@@ -843,7 +878,7 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB
   {
     std::lock_guard<std::mutex> g(mu);
     if (!attr_done[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      const cudaError_t e = cudaFuncSetAttribute(KERN, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
       if (e != cudaSuccess) {
         record_error("cudaFuncSetAttribute", e);
         return MGF_ERR_CUDA;
@@ -851,7 +886,7 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB
       max_units[dev] = 1 << 30;
       if (CG == 2) {  // never more persistent pairs than can be resident at once
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n > 0) max_units[dev] = n;
+        if (cudaOccupancyMaxActiveClusters(&n, KERN, &cfg) == cudaSuccess && n > 0) max_units[dev] = n;
         cudaGetLastError();
       }
       attr_done[dev] = true;
@@ -861,17 +896,30 @@ int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB
   if (tiles < units) units = static_cast<int>(tiles);
   cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
   cudaGetLastError();
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tA, tA32, tB, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, KERN, args...);
   if (e == cudaSuccess && debug_sync()) {
     e = cudaStreamSynchronize(st);
-    fprintf(stderr, "[mgf] block-scaled BN=%d CG=%d epi=%d b_mn=%d units=%d E=%d rows=%lld n=%d k=%d -> %s\n", BN, CG,
-            EPI, int(B_MN), units, p.E, (long long)p.total_rows, p.n, p.k, cudaGetErrorString(e));
+    fprintf(stderr, "[mgf] block-scaled form=%s CG=%d epi=%d b_mn=%d units=%d E=%d rows=%lld n=%d k=%d -> %s\n", form, CG, epi,
+            int(b_mn), units, p.E, (long long)p.total_rows, p.n, p.k, cudaGetErrorString(e));
   }
   if (e != cudaSuccess) {
     record_error("kernel launch", e);
     return MGF_ERR_CUDA;
   }
   return MGF_OK;
+}
+
+template <int EPI, bool B_MN, int CG>
+int launch_mx(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
+  return launch_persistent<mx_kernel<EPI, B_MN, CG>, CG>(MxCfg<CG>::kThreads, MxCfg<CG>::SMEM_BYTES, "mx", EPI, B_MN, p,
+                               tiles, sms, st, tA, tB, p);
+}
+
+template <int BN, int EPI, bool B_MN, int CG>
+int launch(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+           cudaStream_t st) {
+  return launch_persistent<gemm_kernel<BN, EPI, B_MN, CG>, CG>(kThreads, Cfg<BN, CG>::SMEM_BYTES, BN == 128 ? "128" : "256",
+                               EPI, B_MN, p, tiles, sms, st, tA, tA32, tB, p);
 }
 
 template <int BN, int CG>
@@ -890,23 +938,24 @@ int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tA32,
   }
 }
 
+template <int CG>
 int dispatch_mx(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
                 cudaStream_t st) {
   switch (epi) {
     case MGF_EPI_BIAS:
-      return b_mn ? launch_mx<MGF_EPI_BIAS, true>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_BIAS, false>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_BIAS, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_BIAS, false, CG>(tA, tB, p, tiles, sms, st);
     case MGF_EPI_SWIGLU:
-      return b_mn ? launch_mx<MGF_EPI_SWIGLU, true>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_SWIGLU, false>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU, false, CG>(tA, tB, p, tiles, sms, st);
     default:
-      return b_mn ? launch_mx<MGF_EPI_SWIGLU_BWD, true>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_SWIGLU_BWD, false>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU_BWD, true, CG>(tA, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU_BWD, false, CG>(tA, tB, p, tiles, sms, st);
   }
 }
 
-// Workspace of the form with the scales in the tensor cores: packed scales of A (128 rows past the end: a tile reads
-// whole 128-row blocks), of B, and a word per block of the packing kernel.
+// Workspace of the form with the scales in the tensor cores: packed scales of A (256 rows past the end: a tile reads
+// whole 128- or 256-row blocks), of B, and a word per block of the packing kernel.
 constexpr int kPackBlocks = 296;
 struct MxSpace {
   int64_t rows, a_words, b_words;
@@ -915,7 +964,7 @@ struct MxSpace {
 MxSpace mx_space(const mgf_block_gemm_desc& g) {
   const int64_t nkw = ((g.k + BK - 1) / BK + 3) / 4, nnb = (g.n + BK - 1) / BK;
   MxSpace s;
-  s.rows = (g.total_rows + BM + 3) / 4 * 4;
+  s.rows = (g.total_rows + 2 * BM + 3) / 4 * 4;
   s.a_words = nkw * s.rows;
   s.b_words = g.num_groups * nkw * nnb;
   return s;
@@ -1016,6 +1065,9 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   const int64_t groups = g.total_rows < g.num_groups ? g.total_rows : g.num_groups;
   int bn = g.n <= 128 || groups * ((g.n + 255) / 256) < di.sms ? 128 : 256;
   if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
+  // tensor-core scales: pairs from 1024 rows on (SwiGLU backward: 32768 x 7168 x 2048 over 64
+  // groups 565 us single against 588 in pairs, 98304 x 2880 x 5760 over 32 groups 3.33 against 2.19 ms)
+  const int mx_cg = getenv("MGF_CTA_GROUP") != nullptr ? cg : (g.total_rows / g.num_groups >= 1024 ? 2 : 1);
   if (bn == 128) cg = 1;
   p.n_tiles = static_cast<int>((g.n + bn - 1) / bn);
 
@@ -1053,14 +1105,16 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
     pack_scales_kernel<<<kPackBlocks, 256, 0, st>>>(p, ws, ws + sp.a_words, words);
     if (cudaGetLastError() != cudaSuccess) return MGF_ERR_CUDA;
     Params pm = p;
-    pm.n_tiles = static_cast<int>((g.n + MxCfg::BN - 1) / MxCfg::BN);
+    constexpr int kBN = MxCfg<1>::BN;
+    pm.n_tiles = static_cast<int>((g.n + kBN - 1) / kBN);
     CUtensorMap tBm;
-    const uint32_t bBm[3] = {BK, MxCfg::BN, 1};
+    const uint32_t bBm[3] = {BK, static_cast<uint32_t>(kBN / mx_cg), 1};
     if (!encode_bf16(&tBm, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bBm, CU_TENSOR_MAP_SWIZZLE_128B, u8))
       return MGF_ERR_CUDA;
-    const int64_t mx_tiles = (g.total_rows / BM + g.num_groups) * static_cast<int64_t>(pm.n_tiles);
+    const int64_t mx_tiles = (g.total_rows / (BM * mx_cg) + g.num_groups) * static_cast<int64_t>(pm.n_tiles);
     if (mx_tiles > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
-    const int rc = dispatch_mx(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st);
+    const int rc = mx_cg == 2 ? dispatch_mx<2>(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st)
+                              : dispatch_mx<1>(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st);
     if (rc != MGF_OK) return rc;
   }
   if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);

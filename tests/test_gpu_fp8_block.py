@@ -246,24 +246,24 @@ SHAPES = [
 ]
 
 
-@pytest.mark.parametrize("form", ["auto", "single", "pair", "narrow", "choice", "powers"])
+@pytest.mark.parametrize("form", ["auto", "single", "pair", "narrow", "choice", "powers", "powers pair"])
 @pytest.mark.parametrize("layout", ["kn", "nk"])
 @pytest.mark.parametrize("E,K,N,counts", SHAPES)
 def test_products_against_64_bits(E, K, N, counts, layout, form, monkeypatch):
     """auto .. narrow: the launch shapes; choice: arbitrary scales offered to the form that wants powers of two,
-    which has to leave them to the other; powers: powers of two, applied by the tensor cores."""
+    which has to leave them to the other; powers (pair): powers of two, applied by the tensor cores."""
     import cutlass_op.bf16_grouped_mm as m
     from cutlass_op.bf16_grouped_mm import fp8_block
 
-    monkeypatch.setenv("MGF_BLOCK_MX", "1" if form in ("choice", "powers") else "0")
-    if form in ("single", "pair"):
-        monkeypatch.setenv("MGF_CTA_GROUP", "1" if form == "single" else "2")
+    monkeypatch.setenv("MGF_BLOCK_MX", "1" if form.startswith(("choice", "powers")) else "0")
+    if form in ("single", "pair", "powers", "powers pair"):
+        monkeypatch.setenv("MGF_CTA_GROUP", "2" if form.endswith("pair") else "1")
     if form == "narrow":
         monkeypatch.setenv("MGF_BN", "128")
     a, b, offs, sa, sb, bias = _case(E, K, N, counts, layout, E * 7 + K, extra_rows=3)
     rows = int(offs[-1])
     steps = 257 + sa.shape[1]
-    if form == "powers":
+    if form.startswith("powers"):
         steps = 2 * K
         for t in (sa, sb):
             t.copy_(torch.exp2(torch.randint(-6, 7, t.shape, generator=_gen(8), device="cuda").float()))
