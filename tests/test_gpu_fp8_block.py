@@ -378,3 +378,59 @@ def test_product_refusals():
     with pytest.raises(RuntimeError, match="aux"):
         fp8_block.grouped_mm_swiglu_bwd_fp8_block(a, b, offs, torch.zeros(20, 256, device="cuda", dtype=torch.bfloat16),
                                                   sa, sb)
+
+
+@pytest.mark.parametrize("mx", ["0", "1"])
+@pytest.mark.parametrize("cg", ["1", "2"])
+def test_waits_that_run_out_are_reported_and_leave_the_device_usable(mx, cg, monkeypatch):
+    """The launcher's test hook hands out no tiles, so every consumer's bounded wait gives up with nothing in
+    flight; the next launch is right."""
+    from cutlass_op.bf16_grouped_mm import fp8_block
+    from cutlass_op.bf16_grouped_mm._ext import DEV_WAIT_TIMEOUT, device_status
+
+    monkeypatch.setenv("MGF_BLOCK_MX", mx)
+    monkeypatch.setenv("MGF_CTA_GROUP", cg)
+    a, b, offs, sa, sb, bias = _case(2, 256, 256, [130, 10], "kn", 4)
+    sa.fill_(0.5)
+    sb.fill_(2.0)
+    device_status()
+    want = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias)
+    assert device_status() == 0
+    monkeypatch.setenv("MGF_TEST_STALL_PRODUCER", "1")
+    fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias)
+    assert device_status() == DEV_WAIT_TIMEOUT
+    monkeypatch.delenv("MGF_TEST_STALL_PRODUCER")
+    assert torch.equal(fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias), want) and device_status() == 0
+
+
+def test_two_streams_and_a_captured_launch_with_new_scales(monkeypatch):
+    """Two launches at once have scratch of their own; a captured launch chooses its form anew on every replay."""
+    from cutlass_op.bf16_grouped_mm import fp8_block
+
+    monkeypatch.setenv("MGF_BLOCK_MX", "1")
+    a, b, offs, sa, sb, bias = _case(4, 512, 384, [300, 7, 0, 900], "kn", 6)
+    powers = torch.exp2(torch.randint(-3, 4, sa.shape, generator=_gen(1), device="cuda").float())
+    sa1 = torch.empty_strided(sa.shape, sa.stride(), device="cuda").copy_(powers)
+    sb1 = torch.ones_like(sb)
+    f = fp8_block.grouped_mm_fp8_block
+    want = [f(a, b, offs, sa, sb, bias), f(a, b, offs, sa1, sb1, bias)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(4):
+        for s, scales in zip(streams, ((sa, sb), (sa1, sb1))):
+            with torch.cuda.stream(s):
+                got.append(f(a, b, offs, *scales, bias))
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert torch.equal(g, want[i % 2])
+    xa, xb = sa.clone(memory_format=torch.preserve_format), sb.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = f(a, b, offs, xa, xb, bias)
+    for i, scales in ((1, (sa1, sb1)), (0, (sa, sb)), (1, (sa1, sb1))):
+        xa.copy_(scales[0])
+        xb.copy_(scales[1])
+        graph.replay()
+        assert torch.equal(out, want[i])
