@@ -600,7 +600,8 @@ struct MxCfg {
 // rows and of all columns, the even CTA issues.
 template <int EPI, bool B_MN, int CG>
 __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
-    mx_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
+    mx_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmA32,
+              const __grid_constant__ CUtensorMap tmA64, const __grid_constant__ CUtensorMap tmB, const Params p) {
   using C = MxCfg<CG>;
   constexpr int TM = BM * CG;
   constexpr int STAGES = C::STAGES, BN = C::BN, COLS = BN / 2, kSlots = C::kSlots;
@@ -682,6 +683,9 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
       bool ok = true;
       for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
         const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
+        // a tile of few rows loads 32 or 64 rows of A; the products of the stage's other rows are never read
+        const int rows = CG == 2 || ti.row_end - ti.row0 > 64 ? BM : ti.row_end - ti.row0 > 32 ? 64 : 32;
+        const CUtensorMap* map_a = rows == BM ? &tmA : rows == 64 ? &tmA64 : &tmA32;
         for (int kb = 0; kb < nk; ++kb) {
           if (!wait_bounded(ptx::smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag, p.status)) { ok = false; break; }
           uint32_t fb = ptx::smem_u32(&full_bar[stage]);
@@ -689,7 +693,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
             if (leader) ptx::mbar_arrive_expect_tx(fb, 2 * C::STAGE_BYTES);
             else fb = leader_addr(&full_bar[stage]);
           } else {
-            ptx::mbar_arrive_expect_tx(fb, C::STAGE_BYTES);
+            ptx::mbar_arrive_expect_tx(fb, rows * BK + C::BNC * BK);
           }
           const uint32_t sA = ptx::smem_u32(smem + stage * C::STAGE_BYTES), sB = sA + BM * BK;
           const int row = ti.row0 + static_cast<int>(crank) * BM, col = ti.n0 + static_cast<int>(crank) * C::BNC;
@@ -698,7 +702,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
             if constexpr (B_MN) ptx::tma_load_3d_pair(sB, &tmB, fb, col, kb * BK, ti.e);
             else ptx::tma_load_3d_pair(sB, &tmB, fb, kb * BK, col, ti.e);
           } else {
-            ptx::tma_load_2d(sA, &tmA, fb, kb * BK, row);
+            ptx::tma_load_2d(sA, map_a, fb, kb * BK, row);
             if constexpr (B_MN) {
               ptx::tma_load_3d(sB, &tmB, fb, col, kb * BK, ti.e);
               ptx::tma_load_3d(sB + 16384, &tmB, fb, col + 128, kb * BK, ti.e);
@@ -910,9 +914,9 @@ int launch_persistent(int threads, int smem, const char* form, int epi, bool b_m
 }
 
 template <int EPI, bool B_MN, int CG>
-int launch_mx(const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
+int launch_mx(const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tA64, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms, cudaStream_t st) {
   return launch_persistent<mx_kernel<EPI, B_MN, CG>, CG>(MxCfg<CG>::kThreads, MxCfg<CG>::SMEM_BYTES, "mx", EPI, B_MN, p,
-                               tiles, sms, st, tA, tB, p);
+                               tiles, sms, st, tA, tA32, tA64, tB, p);
 }
 
 template <int BN, int EPI, bool B_MN, int CG>
@@ -939,18 +943,19 @@ int dispatch(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tA32,
 }
 
 template <int CG>
-int dispatch_mx(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
+int dispatch_mx(int epi, bool b_mn, const CUtensorMap& tA, const CUtensorMap& tA32, const CUtensorMap& tA64,
+                const CUtensorMap& tB, const Params& p, int64_t tiles, int sms,
                 cudaStream_t st) {
   switch (epi) {
     case MGF_EPI_BIAS:
-      return b_mn ? launch_mx<MGF_EPI_BIAS, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_BIAS, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_BIAS, true, CG>(tA, tA32, tA64, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_BIAS, false, CG>(tA, tA32, tA64, tB, p, tiles, sms, st);
     case MGF_EPI_SWIGLU:
-      return b_mn ? launch_mx<MGF_EPI_SWIGLU, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_SWIGLU, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU, true, CG>(tA, tA32, tA64, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU, false, CG>(tA, tA32, tA64, tB, p, tiles, sms, st);
     default:
-      return b_mn ? launch_mx<MGF_EPI_SWIGLU_BWD, true, CG>(tA, tB, p, tiles, sms, st)
-                  : launch_mx<MGF_EPI_SWIGLU_BWD, false, CG>(tA, tB, p, tiles, sms, st);
+      return b_mn ? launch_mx<MGF_EPI_SWIGLU_BWD, true, CG>(tA, tA32, tA64, tB, p, tiles, sms, st)
+                  : launch_mx<MGF_EPI_SWIGLU_BWD, false, CG>(tA, tA32, tA64, tB, p, tiles, sms, st);
   }
 }
 
@@ -1107,14 +1112,16 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
     Params pm = p;
     constexpr int kBN = MxCfg<1>::BN;
     pm.n_tiles = static_cast<int>((g.n + kBN - 1) / kBN);
-    CUtensorMap tBm;
+    CUtensorMap tA64, tBm;
+    const uint32_t bA64[2] = {BK, 64};
     const uint32_t bBm[3] = {BK, static_cast<uint32_t>(kBN / mx_cg), 1};
-    if (!encode_bf16(&tBm, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bBm, CU_TENSOR_MAP_SWIZZLE_128B, u8))
+    if (!encode_bf16(&tA64, g.a, 2, dA, sA, bA64, CU_TENSOR_MAP_SWIZZLE_128B, u8) ||
+        !encode_bf16(&tBm, g.b, 3, b_mn ? dB_mn : dB_k, sB, b_mn ? bB_mn : bBm, CU_TENSOR_MAP_SWIZZLE_128B, u8))
       return MGF_ERR_CUDA;
     const int64_t mx_tiles = (g.total_rows / (BM * mx_cg) + g.num_groups) * static_cast<int64_t>(pm.n_tiles);
     if (mx_tiles > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
-    const int rc = mx_cg == 2 ? dispatch_mx<2>(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st)
-                              : dispatch_mx<1>(g.epilogue, b_mn, tA, tBm, pm, mx_tiles, sms, st);
+    const int rc = mx_cg == 2 ? dispatch_mx<2>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, sms, st)
+                              : dispatch_mx<1>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, sms, st);
     if (rc != MGF_OK) return rc;
   }
   if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);
