@@ -31,6 +31,7 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kWarps = 8;  // warps per block of the row kernels
 
 // ---------------------------------------------------------------- sort
+constexpr int kFewCopies = 1024;  // up to here sort and permute are one launch
 constexpr int kSortBatch = 8;  // ids a lane loads together (and keeps from pass 1 to pass 2)
 
 // The copies are split into contiguous ranges, one per warp, and every warp keeps its own histogram in
@@ -88,18 +89,19 @@ __global__ void __launch_bounds__(256) count_kernel(const int64_t* __restrict__ 
   for (int e = threadIdx.x; e < E; e += blockDim.x) counts[static_cast<int64_t>(blockIdx.x) * E + e] = smem[e];
 }
 
-// blockDim.x: a multiple of 256, at least E, at most 1024.  counts: of all CTAs, nullptr for one CTA.
-__global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
-                                                    const int32_t* __restrict__ counts, int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
-                                                    int32_t* __restrict__ copy_of_row,
-                                                    unsigned int* __restrict__ status) {
-  extern __shared__ int32_t smem[];
+// Sort of CTA `rank` of `ctas`.  blockDim.x: a multiple of 256, at least E, at most 1024.  smem: (warps + 2) * E words.
+// counts: of all CTAs, nullptr for one CTA.  WRITE: the plan goes to global memory; local_rows (or nullptr): the
+// rows of the copies, [n].  Returns the number of rows.
+template <bool WRITE>
+__device__ __forceinline__ int32_t sort_copies(int32_t* smem, int rank, int ctas, const int64_t* __restrict__ ids, int64_t n,
+                                               int E, const int32_t* __restrict__ counts, int32_t* __restrict__ offs,
+                                               int32_t* __restrict__ row_of_copy, int32_t* __restrict__ copy_of_row,
+                                               int32_t* local_rows, unsigned int* __restrict__ status) {
   const int threads = blockDim.x, warps = threads >> 5;
   int32_t* hist = smem;                // [warps][E]
   int32_t* total = smem + warps * E;   // [E] this CTA's counts
   int32_t* base = total + E;           // [E] first row of this CTA's copies of each expert
   __shared__ int32_t warp_sums[32];
-  const int ctas = gridDim.x, rank = blockIdx.x;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t per_cta = copies_per_cta(n, ctas), per = ((per_cta + warps - 1) / warps + 31) / 32 * 32;
   const int64_t first_copy = rank * per_cta < n ? rank * per_cta : n;
@@ -179,7 +181,7 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ 
   const int32_t first = incl - all + (warp > 0 ? warp_sums[warp - 1] : 0);
   if (threadIdx.x < E) {
     base[threadIdx.x] = first + before;
-    if (rank == 0) offs[threadIdx.x] = first + all;
+    if (WRITE && rank == 0) offs[threadIdx.x] = first + all;
   }
   const int32_t kept = warp_sums[31];
   __syncthreads();
@@ -196,16 +198,30 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ 
       if (id[b] >= 0 && lane == __ffs(same) - 1) mine[id[b]] += __popc(same);
       __syncwarp();
       if (c < end) {
-        row_of_copy[c] = row;
-        if (row >= 0) copy_of_row[row] = static_cast<int32_t>(c);
+        if (WRITE) {
+          row_of_copy[c] = row;
+          if (row >= 0) copy_of_row[row] = static_cast<int32_t>(c);
+        }
+        if (local_rows != nullptr) local_rows[c] = row;
       }
     }
     i += 32 * kSortBatch;
     if (i < end) load_ids(ids, i, end, E, lane, id, bad);
   }
-  for (int64_t r = kept + static_cast<int64_t>(rank) * threads + threadIdx.x; r < n;
-       r += static_cast<int64_t>(ctas) * threads)
-    copy_of_row[r] = -1;
+  if (WRITE)
+    for (int64_t r = kept + static_cast<int64_t>(rank) * threads + threadIdx.x; r < n;
+         r += static_cast<int64_t>(ctas) * threads)
+      copy_of_row[r] = -1;
+  return kept;
+}
+
+__global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
+                                                    const int32_t* __restrict__ counts, int32_t* __restrict__ offs,
+                                                    int32_t* __restrict__ row_of_copy,
+                                                    int32_t* __restrict__ copy_of_row,
+                                                    unsigned int* __restrict__ status) {
+  extern __shared__ int32_t smem[];
+  sort_copies<true>(smem, blockIdx.x, gridDim.x, ids, n, E, counts, offs, row_of_copy, copy_of_row, nullptr, status);
 }
 
 // ---------------------------------------------------------------- row access
@@ -331,6 +347,44 @@ __global__ void __launch_bounds__(32 * kWarps)
     }
   }
   zero_tail<T, VEC>(rows, ldr, n_rows, nv, offs_end);
+}
+
+// Sort and permute of few copies in one launch: every CTA sorts them all for itself (the first one writes the plan),
+// then the CTAs share out the rows.  One launch less on a path that is nothing but launches.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(1024)
+    sort_permute_kernel(const int64_t* __restrict__ ids, int E, const T* __restrict__ x, int64_t ldx, int64_t tokens, int topk,
+                        int64_t nv, int64_t chunks, int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
+                        int32_t* __restrict__ copy_of_row, T* __restrict__ rows, int64_t ldr,
+                        unsigned int* __restrict__ status) {
+  using A = Access<T, VEC>;
+  extern __shared__ int32_t smem[];
+  const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  const int64_t n = tokens * topk;
+  int32_t* row_of = smem + (warps + 2) * E;
+  const int32_t kept = blockIdx.x == 0
+                           ? sort_copies<true>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status)
+                           : sort_copies<false>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status);
+  __syncthreads();
+  const int64_t w0 = static_cast<int64_t>(blockIdx.x) * warps + (threadIdx.x >> 5), nw = static_cast<int64_t>(gridDim.x) * warps;
+  for (int64_t u = w0; u < tokens * chunks; u += nw) {
+    const int64_t t = u / chunks;
+    const int64_t v0 = (u - t * chunks) * (32 * kPermuteVecs) + lane;
+    typename A::Raw r[kPermuteVecs];
+#pragma unroll
+    for (int i = 0; i < kPermuteVecs; ++i)
+      if (v0 + 32 * i < nv) r[i] = A::load(x + t * ldx + (v0 + 32 * i) * A::N);
+    for (int j = 0; j < topk; ++j) {
+      const int32_t row = row_of[t * topk + j];
+      if (row < 0) continue;
+#pragma unroll
+      for (int i = 0; i < kPermuteVecs; ++i)
+        if (v0 + 32 * i < nv) A::store(rows + static_cast<int64_t>(row) * ldr + (v0 + 32 * i) * A::N, r[i]);
+    }
+  }
+  const typename A::Raw z = A::zero();
+  for (int64_t r = kept + w0; r < n; r += nw)
+    for (int64_t v = lane; v < nv; v += 32) A::store(rows + r * ldr + v * A::N, z);
 }
 
 // ---------------------------------------------------------------- unpermute
@@ -541,6 +595,50 @@ extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_ex
   sort_kernel<<<ctas, threads, smem, st>>>(expert_idx, n, num_experts, ctas > 1 ? workspace : nullptr, offs, row_of_copy,
                                            copy_of_row, status);
   return launched();
+}
+
+extern "C" int mgf_moe_sort_permute(const int64_t* expert_idx, int32_t num_experts, const void* x, int32_t dtype,
+                                    int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden, int32_t* offs,
+                                    int32_t* row_of_copy, int32_t* copy_of_row, void* rows, int64_t ldr,
+                                    int32_t* workspace, void* stream) {
+  using namespace mgf;
+  if (topk < 1 || tokens < 0 || tokens > INT32_MAX / topk) return MGF_ERR_INVALID_ARGUMENT;
+  const int64_t n = tokens * topk;
+  if (n == 0 || hidden == 0 || n > kFewCopies) {
+    const int rc = mgf_moe_sort(expert_idx, n, num_experts, offs, row_of_copy, copy_of_row, workspace, stream);
+    if (rc != MGF_OK) return rc;
+    return mgf_moe_permute(x, dtype, ldx, tokens, topk, hidden, row_of_copy, offs + num_experts - 1, rows, ldr, n, stream);
+  }
+  if (!row_args_ok(dtype, tokens, topk, hidden, n) || num_experts < 1 || num_experts > 1024 || expert_idx == nullptr ||
+      x == nullptr || offs == nullptr || row_of_copy == nullptr || copy_of_row == nullptr || rows == nullptr)
+    return MGF_ERR_INVALID_ARGUMENT;
+  unsigned int* status = status_word_address();
+  if (status == nullptr) return MGF_ERR_CUDA;
+  const int es = elem_size(dtype);
+  const bool vec = (hidden * es) % 16 == 0 && vec_ok(x, ldx, es) && vec_ok(rows, ldr, es);
+  return for_type(dtype, vec, [&](auto e, auto v) {
+    using T = decltype(e);
+    constexpr bool VEC = decltype(v)::value;
+    auto kern = sort_permute_kernel<T, VEC>;
+    const int smem_most = static_cast<int>((34 * 1024 + kFewCopies) * sizeof(int32_t));
+    static std::atomic<bool> attr_done[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return static_cast<int>(MGF_ERR_CUDA);
+    if (!attr_done[dev]) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_most) != cudaSuccess)
+        return static_cast<int>(MGF_ERR_CUDA);
+      attr_done[dev] = true;
+    }
+    const unsigned threads = (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
+    const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 32 * kPermuteVecs - 1) / (32 * kPermuteVecs);
+    const int64_t blocks = (tokens * chunks * 32 + threads - 1) / threads;
+    const unsigned grid = static_cast<unsigned>(blocks < 296 ? blocks : 296);
+    const size_t smem = (static_cast<size_t>(threads / 32 + 2) * num_experts + n) * sizeof(int32_t);
+    kern<<<grid, threads, smem, static_cast<cudaStream_t>(stream)>>>(
+        expert_idx, num_experts, static_cast<const T*>(x), ldx, tokens, topk, nv, chunks, offs, row_of_copy, copy_of_row,
+        static_cast<T*>(rows), ldr, status);
+    return launched();
+  });
 }
 
 extern "C" int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden,

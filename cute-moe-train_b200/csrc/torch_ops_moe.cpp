@@ -116,24 +116,39 @@ void check_experts(int64_t num_experts) {
               num_experts);
 }
 
-std::tuple<Tensor, Tensor, Tensor> moe_sort_cuda(const Tensor& expert_idx, int64_t num_experts) {
+void check_ids(const Tensor& expert_idx, int64_t num_experts) {
   TORCH_CHECK(expert_idx.is_cuda() && expert_idx.scalar_type() == at::kLong && expert_idx.dim() == 2 &&
                   expert_idx.size(1) >= 1 && expert_idx.is_contiguous(),
               "moe_sort: expert_idx must be a contiguous int64 [tokens, topk] CUDA tensor");
   check_experts(num_experts);
-  const int64_t n = expert_idx.numel();
-  TORCH_CHECK(n <= kMaxCopies, "moe_sort: too many copies, ", n);
-  const c10::cuda::CUDAGuard guard(expert_idx.device());
+  TORCH_CHECK(expert_idx.numel() <= kMaxCopies, "moe_sort: too many copies, ", expert_idx.numel());
+}
+
+struct Plan {
+  Tensor offs, row_of_copy, copy_of_row, workspace;
+  int32_t* scratch = nullptr;
+};
+
+Plan empty_plan(const Tensor& expert_idx, int64_t num_experts) {
   const auto o = expert_idx.options().dtype(at::kInt);
-  Tensor offs = at::empty({num_experts}, o), row_of_copy = at::empty(expert_idx.sizes(), o), copy_of_row = at::empty({n}, o);
-  Tensor ws;
-  const int64_t words = mgf_moe_sort_workspace_words(n, static_cast<int32_t>(num_experts));
-  if (words > 0) ws = at::empty({words}, o);
-  check_launch(mgf_moe_sort(expert_idx.data_ptr<int64_t>(), n, static_cast<int32_t>(num_experts),
-                            offs.data_ptr<int32_t>(), row_of_copy.data_ptr<int32_t>(), copy_of_row.data_ptr<int32_t>(),
-                            words > 0 ? ws.data_ptr<int32_t>() : nullptr, stream()),
+  const int64_t n = expert_idx.numel(), words = mgf_moe_sort_workspace_words(n, static_cast<int32_t>(num_experts));
+  Plan p{at::empty({num_experts}, o), at::empty(expert_idx.sizes(), o), at::empty({n}, o), Tensor()};
+  if (words > 0) {
+    p.workspace = at::empty({words}, o);
+    p.scratch = p.workspace.data_ptr<int32_t>();
+  }
+  return p;
+}
+
+std::tuple<Tensor, Tensor, Tensor> moe_sort_cuda(const Tensor& expert_idx, int64_t num_experts) {
+  check_ids(expert_idx, num_experts);
+  const c10::cuda::CUDAGuard guard(expert_idx.device());
+  Plan p = empty_plan(expert_idx, num_experts);
+  check_launch(mgf_moe_sort(expert_idx.data_ptr<int64_t>(), expert_idx.numel(), static_cast<int32_t>(num_experts),
+                            p.offs.data_ptr<int32_t>(), p.row_of_copy.data_ptr<int32_t>(),
+                            p.copy_of_row.data_ptr<int32_t>(), p.scratch, stream()),
                "moe_sort");
-  return {offs, row_of_copy, copy_of_row};
+  return {p.offs, p.row_of_copy, p.copy_of_row};
 }
 
 void check_plan(const Tensor& offs, const Tensor& row_of_copy, const Tensor& like, const char* what) {
@@ -170,8 +185,18 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_permute_cuda(const Tensor& x, con
   TORCH_CHECK(expert_idx.device() == x.device(), "moe_permute: expert_idx must be on x's device");
   TORCH_CHECK(expert_idx.dim() == 2 && expert_idx.size(0) == x.size(0),
               "moe_permute: expert_idx must be [tokens, topk] for the tokens of x");
-  auto [offs, row_of_copy, copy_of_row] = moe_sort_cuda(expert_idx, num_experts);
-  return {permute_rows_cuda(x, offs, row_of_copy), offs, row_of_copy, copy_of_row};
+  const int32_t dt = dtype_code(x, "moe_permute");
+  check_ids(expert_idx, num_experts);
+  const c10::cuda::CUDAGuard guard(x.device());
+  Plan p = empty_plan(expert_idx, num_experts);
+  Tensor rows = padded_rows(expert_idx.numel(), x.size(1), x.options());
+  check_launch(mgf_moe_sort_permute(expert_idx.data_ptr<int64_t>(), static_cast<int32_t>(num_experts), x.data_ptr(), dt,
+                                    row_stride(x), x.size(0), static_cast<int32_t>(expert_idx.size(1)), x.size(1),
+                                    p.offs.data_ptr<int32_t>(), p.row_of_copy.data_ptr<int32_t>(),
+                                    p.copy_of_row.data_ptr<int32_t>(), rows.data_ptr(), rows.stride(0), p.scratch,
+                                    stream()),
+               "moe_permute");
+  return {rows, p.offs, p.row_of_copy, p.copy_of_row};
 }
 
 void check_weights(const std::optional<Tensor>& weights, const Tensor& row_of_copy) {

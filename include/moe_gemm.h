@@ -282,12 +282,16 @@ int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int3
  * width allow).  offs_end points at offs[E-1].  A row index >= n_rows is skipped and sets
  * MGF_DEV_ROW_OUT_OF_RANGE.
  *   permute:       rows[row_of_copy[t*topk+j]] = x[t]; rows from *offs_end to n_rows become zeros
+ *   sort_permute:  mgf_moe_sort and permute (n_rows = tokens * topk) in one call; one launch for few copies
  *   unpermute:     out[t] = sum_j weights[t*topk+j] * rows[row_of_copy[t*topk+j]]  (fp32 sum; NULL weights: 1)
  *   unpermute_bwd: grad_rows[row] = weight * grad_out[t] (rows behind *offs_end: zeros) and
  *                  grad_weights[t*topk+j] = <rows[row], grad_out[t]> (0 for a dropped copy); either may be NULL. */
 int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_t tokens, int32_t topk, int64_t hidden,
                     const int32_t* row_of_copy, const int32_t* offs_end, void* rows, int64_t ldr, int64_t n_rows,
                     void* stream);
+int mgf_moe_sort_permute(const int64_t* expert_idx, int32_t num_experts, const void* x, int32_t dtype, int64_t ldx,
+                         int64_t tokens, int32_t topk, int64_t hidden, int32_t* offs, int32_t* row_of_copy,
+                         int32_t* copy_of_row, void* rows, int64_t ldr, int32_t* workspace, void* stream);
 int mgf_moe_unpermute(const void* rows, int32_t dtype, int64_t ldr, int64_t n_rows, int64_t tokens, int32_t topk,
                       int64_t hidden, const int32_t* row_of_copy, const float* weights, void* out, int64_t ldo,
                       void* stream);
