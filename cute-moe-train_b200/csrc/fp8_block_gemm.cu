@@ -544,8 +544,16 @@ __global__ void __launch_bounds__(256) pack_scales_kernel(const Params p, uint32
     other |= (b & 0x807FFFFFu) != 0u || e == 0u || e == 255u;
     return e & 0xffu;
   };
-  int64_t rows = __ldg(p.offs + p.E - 1);
-  rows = rows < 0 ? 0 : (rows > p.total_rows ? p.total_rows : rows);
+  // the largest end, not the last one: decreasing offs are clamped by the products, whose rows need their scales too
+  __shared__ int last_row;
+  if (threadIdx.x == 0) last_row = 0;
+  __syncthreads();
+  int most = 0;
+  for (int e = threadIdx.x; e < p.E; e += blockDim.x) most = max(most, __ldg(p.offs + e));
+  most = __reduce_max_sync(0xffffffffu, most);
+  if ((threadIdx.x & 31) == 0) atomicMax(&last_row, most);
+  __syncthreads();
+  const int64_t rows = last_row < p.total_rows ? last_row : p.total_rows;
   const bool vec = (reinterpret_cast<uintptr_t>(p.scale_a) & 15u) == 0 && p.lds_a % 4 == 0;
   for (int64_t r = t0; r < rows; r += nt) {
     const float* s = p.scale_a + r * p.lds_a;

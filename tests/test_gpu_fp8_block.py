@@ -339,16 +339,27 @@ def test_rows_behind_the_last_group_stay_as_they_were():
     assert torch.equal(out[:135], want[:135]) and (out[135:] == 7.0).all()
 
 
-def test_malformed_offs_are_clamped_and_reported():
+def test_malformed_offs_are_clamped_and_reported(monkeypatch):
     from cutlass_op.bf16_grouped_mm import fp8_block
     from cutlass_op.bf16_grouped_mm._ext import DEV_BAD_OFFS, device_status
 
     device_status()
     a, b, offs, sa, sb, _ = _case(3, 128, 128, [10, 10, 10], "kn", 2)
-    good = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb)
-    bad = torch.tensor([10, 20, 5000], dtype=torch.int32, device="cuda")
-    assert torch.equal(fp8_block.grouped_mm_fp8_block(a, b, bad, sa, sb), good)
-    assert device_status() == DEV_BAD_OFFS
+    for mx in ("0", "1"):
+        monkeypatch.setenv("MGF_BLOCK_MX", mx)
+        if mx == "1":
+            sa.fill_(0.25), sb.fill_(4.0)
+        good = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb)
+        bad = torch.tensor([10, 20, 5000], dtype=torch.int32, device="cuda")
+        assert torch.equal(fp8_block.grouped_mm_fp8_block(a, b, bad, sa, sb), good)
+        assert device_status() == DEV_BAD_OFFS
+        # decreasing: group 0 has rows 0 .. 19, the others none
+        bad = torch.tensor([20, 10, 5], dtype=torch.int32, device="cuda")
+        fixed = torch.tensor([20, 20, 20], dtype=torch.int32, device="cuda")
+        want = fp8_block.grouped_mm_fp8_block(a, b, fixed, sa, sb)[:20]
+        assert device_status() == 0
+        assert torch.equal(fp8_block.grouped_mm_fp8_block(a, b, bad, sa, sb)[:20], want)
+        assert device_status() == DEV_BAD_OFFS
 
 
 def test_product_refusals():

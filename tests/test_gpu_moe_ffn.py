@@ -196,3 +196,41 @@ def test_block_refusals_and_empty_batch():
         assert out.shape == (0, 128)
         for gr, t in zip(torch.autograd.grad(out.sum(), leaves), leaves):
             assert gr.shape == t.shape and (gr == 0).all()
+
+
+def test_block_through_a_tracing_compiler():
+    """Fake tensors and autograd of every operator agree with what runs (traced forward and backward)."""
+    from cutlass_op.bf16_grouped_mm.permute import MoEPlan
+    from cutlass_op.bf16_grouped_mm.routing import moe_route
+
+    ops = torch.ops.grouped_mm
+    w = _params(4, 64, 32, 1)
+    x = torch.randn(6, 64, generator=_gen(1), device="cuda").to(torch.bfloat16)
+    logits = torch.randn(6, 4, generator=_gen(2), device="cuda")
+    wt, idx = moe_route(logits, 2)
+    rows, *plan = ops.moe_permute(x, idx, 4)
+    plan = MoEPlan(*plan)
+    lg, xg, rg, wg = (t.detach().clone().requires_grad_(True) for t in (logits, x, rows, wt))
+    checks = ["test_schema", "test_autograd_registration", "test_faketensor"]
+    for op, args in ((ops.moe_route, (lg, 2, 0, True, 1.0, None, None)), (ops.moe_route, (logits, 2, 1, False, 2.0, None, None)),
+                     (ops.moe_sort, (idx, 4)), (ops.moe_permute, (xg, idx, 4)),
+                     (ops.moe_permute_rows, (xg, plan.offs, plan.row_of_copy)),
+                     (ops.moe_unpermute, (rg, plan.offs, plan.row_of_copy, wg)),
+                     (ops.moe_unpermute, (rows, plan.offs, plan.row_of_copy, None)),
+                     (ops.fp8_quantize_rows_block, (x,)), (ops.fp8_quantize_weights_block, (w[0],)),
+                     (ops.fp8_quantize_weights_block, (w[0].transpose(1, 2),)),
+                     (ops.moe_permute_fp8, (x, idx, 4))):
+        torch.library.opcheck(op.default, args, test_utils=checks)
+
+    def step(lg, xg):
+        wt, idx = ops.moe_route(lg, 2, 0, True, 1.0, None, None)
+        rows, offs, row_of_copy, _ = ops.moe_permute(xg, idx, 4)
+        return ops.moe_unpermute(rows * 2, offs, row_of_copy, wt)
+
+    go = torch.randn(6, 64, generator=_gen(3), device="cuda").to(torch.bfloat16)
+    want = step(lg, xg)
+    ref = torch.autograd.grad(want, (lg, xg), go)
+    out = torch.compile(step, backend="aot_eager", fullgraph=True)(lg, xg)
+    assert torch.equal(out, want)
+    for a, b in zip(torch.autograd.grad(out, (lg, xg), go), ref):
+        assert torch.equal(a, b)
