@@ -51,7 +51,7 @@ def quantize_rows_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     x[m, k] ~= q[m, k] * scale[m, k // 128].  Non-finite elements become NaN codes and do not enter their
     block's scale."""
     with timed("fp8_quantize"):
-        return torch.ops.grouped_mm.fp8_quantize_rows_block(x.detach())
+        return torch.ops.grouped_mm.fp8_quantize_rows_block.default(x.detach())
 
 
 def quantize_weights_block(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -59,7 +59,7 @@ def quantize_weights_block(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]
     [E, ceil(K / 128), ceil(N / 128)]): w[e, k, n] ~= q[e, k, n] * scale[e, k // 128, n // 128].
     ``q.transpose(1, 2), scale.transpose(1, 2)`` are the codes of ``w.transpose(1, 2)``."""
     with timed("fp8_quantize"):
-        return torch.ops.grouped_mm.fp8_quantize_weights_block(w.detach())
+        return torch.ops.grouped_mm.fp8_quantize_weights_block.default(w.detach())
 
 
 def dequantize_rows_block(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
@@ -101,7 +101,7 @@ def grouped_mm_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.T
     offs int32 [E] cumulative row ends, N a multiple of 8.  Rows behind offs[-1] are not written.
     """
     with timed("fp8_block_mm"):
-        return torch.ops.grouped_mm.mm_fp8_block(mat_a, mat_b, offs, scale_a, scale_b, bias)
+        return torch.ops.grouped_mm.mm_fp8_block.default(mat_a, mat_b, offs, scale_a, scale_b, bias)
 
 
 def grouped_mm_swiglu_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.Tensor, scale_a: torch.Tensor,
@@ -110,7 +110,7 @@ def grouped_mm_swiglu_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: 
     """The product + bias + clamped SwiGLU -> (swiglu_out [total_M, I], aux_biased_acc [total_M, 2I]), the
     activation computed from the stored (bf16) aux; mat_b's columns interleave gate and up."""
     with timed("fp8_block_up_swiglu_fwd"):
-        return torch.ops.grouped_mm.mm_swiglu_fp8_block(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha,
+        return torch.ops.grouped_mm.mm_swiglu_fp8_block.default(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha,
                                                         swiglu_limit)
 
 
@@ -120,7 +120,7 @@ def grouped_mm_swiglu_bwd_fp8_block(grad_output: torch.Tensor, down_w_t: torch.T
     """SwiGLU backward of the product grad_output @ down_w_t against aux -> grad_aux bf16 [total_M, 2I]
     (interleaved like aux)."""
     with timed("fp8_block_down_dgrad_swiglu_bwd"):
-        return torch.ops.grouped_mm.mm_swiglu_bwd_fp8_block(grad_output, down_w_t, offs, aux_biased_acc, scale_a,
+        return torch.ops.grouped_mm.mm_swiglu_bwd_fp8_block.default(grad_output, down_w_t, offs, aux_biased_acc, scale_a,
                                                             scale_b, swiglu_alpha, swiglu_limit)
 
 

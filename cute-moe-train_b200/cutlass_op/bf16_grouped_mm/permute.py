@@ -97,7 +97,7 @@ def moe_sort(expert_idx: torch.Tensor, num_experts: int) -> MoEPlan:
     num_experts <= 1024.
     """
     with timed("moe_sort"):
-        return MoEPlan(*torch.ops.grouped_mm.moe_sort(expert_idx, num_experts))
+        return MoEPlan(*torch.ops.grouped_mm.moe_sort.default(expert_idx, num_experts))
 
 
 def moe_permute(x: torch.Tensor, expert_idx: torch.Tensor | None = None, num_experts: int | None = None,
@@ -109,10 +109,10 @@ def moe_permute(x: torch.Tensor, expert_idx: torch.Tensor | None = None, num_exp
     """
     with timed("moe_permute"):
         if plan is not None:
-            return torch.ops.grouped_mm.moe_permute_rows(x, plan.offs, plan.row_of_copy), plan
+            return torch.ops.grouped_mm.moe_permute_rows.default(x, plan.offs, plan.row_of_copy), plan
         if expert_idx is None or num_experts is None:
             raise ValueError("moe_permute needs expert_idx and num_experts, or a plan")
-        rows, *p = torch.ops.grouped_mm.moe_permute(x, expert_idx, num_experts)
+        rows, *p = torch.ops.grouped_mm.moe_permute.default(x, expert_idx, num_experts)
         return rows, MoEPlan(*p)
 
 
@@ -123,10 +123,10 @@ def moe_permute_fp8(x: torch.Tensor, expert_idx: torch.Tensor | None = None, num
     have zero codes and scales.  No autograd: the codes feed inference, or a backward that uses x."""
     with timed("moe_permute_fp8"):
         if plan is not None:
-            return (*torch.ops.grouped_mm.moe_permute_rows_fp8(x.detach(), plan.offs, plan.row_of_copy), plan)
+            return (*torch.ops.grouped_mm.moe_permute_rows_fp8.default(x.detach(), plan.offs, plan.row_of_copy), plan)
         if expert_idx is None or num_experts is None:
             raise ValueError("moe_permute_fp8 needs expert_idx and num_experts, or a plan")
-        q, scale, *p = torch.ops.grouped_mm.moe_permute_fp8(x.detach(), expert_idx, num_experts)
+        q, scale, *p = torch.ops.grouped_mm.moe_permute_fp8.default(x.detach(), expert_idx, num_experts)
         return q, scale, MoEPlan(*p)
 
 
@@ -134,4 +134,4 @@ def moe_unpermute(rows: torch.Tensor, plan: MoEPlan, weights: torch.Tensor | Non
     """out[t] = sum_j weights[t, j] * rows[plan.row_of_copy[t, j]] (weights fp32 [tokens, topk], or 1),
     summed in fp32 and rounded once.  Gradients: rows and weights, from one pass over the rows."""
     with timed("moe_unpermute"):
-        return torch.ops.grouped_mm.moe_unpermute(rows, plan.offs, plan.row_of_copy, weights)
+        return torch.ops.grouped_mm.moe_unpermute.default(rows, plan.offs, plan.row_of_copy, weights)

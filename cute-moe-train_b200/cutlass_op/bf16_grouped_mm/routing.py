@@ -53,4 +53,4 @@ def moe_route(logits: torch.Tensor, topk: int, score: str = "softmax", renormali
     if score not in _SCORES:
         raise ValueError(f"moe_route: score must be one of {sorted(_SCORES)}, got {score!r}")
     with timed("moe_route"):
-        return torch.ops.grouped_mm.moe_route(logits, topk, _SCORES[score], renormalize, scale, bias, token_mask)
+        return torch.ops.grouped_mm.moe_route.default(logits, topk, _SCORES[score], renormalize, scale, bias, token_mask)
