@@ -95,7 +95,7 @@ def check_device_status(device: int | None = None) -> None:
         if st & DEV_BAD_OFFS:
             what.append("offs was not non-decreasing within [0, total rows]")
         if st & DEV_ROW_OUT_OF_RANGE:
-            what.append("a gather/combine/push/permute row index or an expert id fell outside its range (row skipped)")
+            what.append("a gather/combine/push/permute row index fell outside its buffer, or an expert id its range (row skipped)")
         raise RuntimeError("grouped_mm device status: " + "; ".join(what))
 
 
