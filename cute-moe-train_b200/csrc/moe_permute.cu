@@ -349,6 +349,53 @@ __global__ void __launch_bounds__(32 * kWarps)
   zero_tail<T, VEC>(rows, ldr, n_rows, nv, offs_end);
 }
 
+// Sort of up to 256 copies by counting: a copy's row is the number of copies with a smaller id or with its own id and
+// before it, a thread per copy; offs[e] is the number with an id up to e, a thread per expert.  No histogram, no scan and
+// one barrier (decode permutation, 32 copies: 3.8 us against 4.7).  ids_s: shared memory, a multiple of 4 words.
+constexpr int kCountedCopies = 256;
+
+template <bool WRITE>
+__device__ __forceinline__ int32_t count_copies(int32_t* ids_s, const int64_t* __restrict__ ids, int n, int E,
+                                                int32_t* __restrict__ offs, int32_t* __restrict__ row_of_copy,
+                                                int32_t* __restrict__ copy_of_row, int32_t* local_rows,
+                                                unsigned int* __restrict__ status) {
+  const int c = threadIdx.x, n4 = (n + 3) / 4 * 4;
+  int mine = E;  // dropped copies sort behind all experts
+  if (c < n) {
+    const int64_t v = __ldg(ids + c);
+    if (v >= 0 && v < E) mine = static_cast<int>(v);
+    else if (v != -1) atomicOr(status, MGF_DEV_ROW_OUT_OF_RANGE);
+  }
+  if (c < n4) ids_s[c] = mine;
+  const int32_t kept = __syncthreads_count(mine < E);
+  const int4* all = reinterpret_cast<const int4*>(ids_s);
+  if (c < n) {
+    int row = 0;
+    for (int i = 0; i < n4 / 4; ++i) {
+      const int4 v = all[i];
+      row += (v.x < mine || (v.x == mine && 4 * i < c)) + (v.y < mine || (v.y == mine && 4 * i + 1 < c)) +
+             (v.z < mine || (v.z == mine && 4 * i + 2 < c)) + (v.w < mine || (v.w == mine && 4 * i + 3 < c));
+    }
+    if (mine == E) row = -1;
+    local_rows[c] = row;
+    if (WRITE) {
+      row_of_copy[c] = row;
+      if (row >= 0) copy_of_row[row] = c;
+      if (c >= kept) copy_of_row[c] = -1;
+    }
+  }
+  if (WRITE)
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+      int end = 0;
+      for (int i = 0; i < n4 / 4; ++i) {
+        const int4 v = all[i];
+        end += (v.x <= e) + (v.y <= e) + (v.z <= e) + (v.w <= e);
+      }
+      offs[e] = end;
+    }
+  return kept;
+}
+
 // Sort and permute of few copies in one launch: every CTA sorts them all for itself (the first one writes the plan),
 // then the CTAs share out the rows.  One launch less on a path that is nothing but launches.
 template <typename T, bool VEC>
@@ -361,10 +408,15 @@ __global__ void __launch_bounds__(1024)
   extern __shared__ int32_t smem[];
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t n = tokens * topk;
-  int32_t* row_of = smem + (warps + 2) * E;
-  const int32_t kept = blockIdx.x == 0
-                           ? sort_copies<true>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status)
-                           : sort_copies<false>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status);
+  int32_t* row_of = smem + (n <= kCountedCopies ? kCountedCopies : (warps + 2) * E);
+  int32_t kept;
+  if (n <= kCountedCopies)
+    kept = blockIdx.x == 0 ? count_copies<true>(smem, ids, n, E, offs, row_of_copy, copy_of_row, row_of, status)
+                           : count_copies<false>(smem, ids, n, E, offs, row_of_copy, copy_of_row, row_of, status);
+  else
+    kept = blockIdx.x == 0
+               ? sort_copies<true>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status)
+               : sort_copies<false>(smem, 0, 1, ids, n, E, nullptr, offs, row_of_copy, copy_of_row, row_of, status);
   __syncthreads();
   const int64_t w0 = static_cast<int64_t>(blockIdx.x) * warps + (threadIdx.x >> 5), nw = static_cast<int64_t>(gridDim.x) * warps;
   for (int64_t u = w0; u < tokens * chunks; u += nw) {
@@ -634,11 +686,12 @@ extern "C" int mgf_moe_sort_permute(const int64_t* expert_idx, int32_t num_exper
         return static_cast<int>(MGF_ERR_CUDA);
       attr_done[dev] = true;
     }
-    const unsigned threads = (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
+    const unsigned threads = n <= kCountedCopies ? 256u : (static_cast<unsigned>(num_experts) + 255u) / 256u * 256u;
     const int64_t nv = hidden / Access<T, VEC>::N, chunks = (nv + 32 * kPermuteVecs - 1) / (32 * kPermuteVecs);
     const int64_t blocks = (tokens * chunks * 32 + threads - 1) / threads;
     const unsigned grid = static_cast<unsigned>(blocks < 296 ? blocks : 296);
-    const size_t smem = (static_cast<size_t>(threads / 32 + 2) * num_experts + n) * sizeof(int32_t);
+    const size_t plan_words = n <= kCountedCopies ? kCountedCopies : (threads / 32 + 2) * static_cast<size_t>(num_experts);
+    const size_t smem = (plan_words + n) * sizeof(int32_t);
     kern<<<grid, threads, smem, static_cast<cudaStream_t>(stream)>>>(
         expert_idx, num_experts, static_cast<const T*>(x), ldx, tokens, topk, nv, chunks, offs, row_of_copy, copy_of_row,
         static_cast<T*>(rows), ldr, status);

@@ -243,6 +243,20 @@ def test_sort_of_many_copies(n, E):
     assert torch.equal(plan.row_of_copy.flatten().long(), inv)
 
 
+@pytest.mark.parametrize("T,k,E,drop", [(1, 1, 1, 0), (8, 4, 32, 0), (64, 4, 1024, 0.3), (257, 1, 5, 0.2), (250, 4, 3, 0.1),
+                                          (128, 8, 1000, 0), (3, 5, 2, 1.1), (1025, 1, 9, 0.1)])
+def test_permute_sorts_as_the_sort_does(T, k, E, drop):
+    """Few copies are sorted within the permuting launch; the plan is the same."""
+    from cutlass_op.bf16_grouped_mm.permute import moe_permute, moe_sort
+
+    idx = _ids(_gen(T * 7 + E), T, k, E, drop)
+    x = torch.randn(T, 24, generator=_gen(1), device="cuda")
+    rows, plan = moe_permute(x, idx, E)
+    for a, b in zip(plan, moe_sort(idx, E)):
+        assert torch.equal(a, b)
+    assert torch.equal(rows, moe_permute(x, plan=plan)[0])
+
+
 def test_sort_reports_ids_out_of_range_and_drops_them():
     import cutlass_op.bf16_grouped_mm as m
     from cutlass_op.bf16_grouped_mm._ext import DEV_ROW_OUT_OF_RANGE, device_status
@@ -253,6 +267,12 @@ def test_sort_reports_ids_out_of_range_and_drops_them():
     assert device_status() == DEV_ROW_OUT_OF_RANGE
     assert plan.offs.tolist() == [1, 2] and plan.row_of_copy.tolist() == [[0, -1], [-1, 1]]
     assert plan.copy_of_row.tolist() == [0, 3, -1, -1]
+    from cutlass_op.bf16_grouped_mm.permute import moe_permute
+
+    x = torch.tensor([[1.0], [2.0]], device="cuda")
+    rows, same = moe_permute(x, torch.tensor([[0, 5], [-2, 1]], device="cuda"), 2)
+    assert device_status() == DEV_ROW_OUT_OF_RANGE
+    assert all(torch.equal(a, b) for a, b in zip(same, plan)) and rows.flatten().tolist() == [1.0, 2.0, 0.0, 0.0]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
