@@ -199,27 +199,36 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
 }
 
 // Sigmoid from the exponential (relative error a few 2^-23): the tanh form's absolute error of about 2^-12
-// would be a relative error of tens of percent at gates of -4.
-__device__ __forceinline__ float sigmoid(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
-__device__ __forceinline__ float swiglu(float g, float u, float alpha, float limit) {
-  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
-  return gc * sigmoid(alpha * gc) * (uc + 1.0f);
+// would be a relative error of tens of percent at gates of -4.  neg_alpha_log2e = -alpha * log2(e).
+__device__ __forceinline__ float sigmoid(float gate, float neg_alpha_log2e) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(gate * neg_alpha_log2e));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return r;
 }
-__device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, float alpha, float limit) {
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float swiglu(float g, float u, float neg_alpha_log2e, float limit) {
+  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
+  return gc * sigmoid(gc, neg_alpha_log2e) * (uc + 1.0f);
+}
+// d_gate = gs (uc + 1) sig (1 + alpha gc (1 - sig)), d_up = gs gc sig, each 0 where its input is clamped.
+__device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, float alpha, float neg_alpha_log2e, float limit) {
   const float g = bf16_lo(aux_word), u = bf16_hi(aux_word);
   const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
-  const float sig = sigmoid(alpha * gc);
-  const float d_gate = (g <= limit) ? gs * (uc + 1.0f) * sig * (1.0f + alpha * gc * (1.0f - sig)) : 0.0f;
-  const float d_up = (u >= -limit && u <= limit) ? gs * gc * sig : 0.0f;
+  const float sig = sigmoid(gc, neg_alpha_log2e), t = gs * sig;
+  const float d_gate = g <= limit ? t * (uc + 1.0f) * fmaf(alpha * gc, 1.0f - sig, 1.0f) : 0.0f;
+  const float d_up = fabsf(u) <= limit ? t * gc : 0.0f;
   return pack_bf16x2(d_gate, d_up);
 }
 
 // Epilogue of one row's COLS columns from column c0 on.  AHEAD (SWIGLU_BWD): aw holds the first 32 columns' aux words
-// and every chunk's are loaded one chunk ahead; otherwise they are loaded where they are used (fewer registers).
+// and every chunk's are loaded one chunk ahead (two ahead: no gain); otherwise they are loaded where they are used
+// (fewer registers).
 template <int EPI, int COLS, bool AHEAD>
 __device__ __forceinline__ void write_columns(const Params& p, const float (&acc)[COLS], int e, int grow, int c0,
                                               uint4 (&aw)[8]) {
+  const float nal = -p.alpha * kLog2e;
   // 32 columns at a time; n is a multiple of 8 (SWIGLU: 16), so units of 8 columns are whole
 #pragma unroll
   for (int c = 0; c < COLS / 32; ++c) {
@@ -244,10 +253,10 @@ __device__ __forceinline__ void write_columns(const Params& p, const float (&acc
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float* f = acc + c * 32 + 4 * (g + h);
-            o[h].x = swiglu_bwd(f[0], cur[g + h].x, p.alpha, p.limit);
-            o[h].y = swiglu_bwd(f[1], cur[g + h].y, p.alpha, p.limit);
-            o[h].z = swiglu_bwd(f[2], cur[g + h].z, p.alpha, p.limit);
-            o[h].w = swiglu_bwd(f[3], cur[g + h].w, p.alpha, p.limit);
+            o[h].x = swiglu_bwd(f[0], cur[g + h].x, p.alpha, nal, p.limit);
+            o[h].y = swiglu_bwd(f[1], cur[g + h].y, p.alpha, nal, p.limit);
+            o[h].z = swiglu_bwd(f[2], cur[g + h].z, p.alpha, nal, p.limit);
+            o[h].w = swiglu_bwd(f[3], cur[g + h].w, p.alpha, nal, p.limit);
           }
           if (p.d_v8) ptx::st_v8(gp + g, o[0], o[1]);
           else {
@@ -280,8 +289,8 @@ __device__ __forceinline__ void write_columns(const Params& p, const float (&acc
 #pragma unroll
         for (int h = 0; h < 8; ++h)
           so[h] = pack_bf16x2(
-              swiglu(bf16_lo(packed[2 * h]), bf16_hi(packed[2 * h]), p.alpha, p.limit),
-              swiglu(bf16_lo(packed[2 * h + 1]), bf16_hi(packed[2 * h + 1]), p.alpha, p.limit));
+              swiglu(bf16_lo(packed[2 * h]), bf16_hi(packed[2 * h]), nal, p.limit),
+              swiglu(bf16_lo(packed[2 * h + 1]), bf16_hi(packed[2 * h + 1]), nal, p.limit));
         const uint4 us[2] = {make_uint4(so[0], so[1], so[2], so[3]), make_uint4(so[4], so[5], so[6], so[7])};
         store_units<2>(p.d2 + (int64_t)grow * p.ldd2 + (col0 >> 1), us, (p.n - col0) >> 4, p.d2_v8);
       }
