@@ -992,8 +992,9 @@ MxSpace mx_space(const mgf_block_gemm_desc& g) {
   return s;
 }
 
-// The tensor cores' scales save the promotion but cost two small launches (packing; the form that returns at
-// once).  MGF_BLOCK_MX=0|1 forces a choice.
+// The tensor cores' scales save the promotion but cost two small launches (packing 5-10 us, the form that returns at
+// once 2.5 us).  From 1024 rows on (n = 5760, k = 2880, 32 groups, SwiGLU: 111 against 114 us at 1024 rows, 143 against 158
+// at 4096; at 256 rows 96 against 98, at 32 rows 70 against 59).  MGF_BLOCK_MX=0|1 forces a choice.
 bool use_mx(const mgf_block_gemm_desc& g) {
   if (const char* env = getenv("MGF_BLOCK_MX"); env != nullptr && (env[0] == '0' || env[0] == '1')) return env[0] == '1';
   return g.n > 128 && g.total_rows >= 1024;
@@ -1087,8 +1088,8 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   const int64_t groups = g.total_rows < g.num_groups ? g.total_rows : g.num_groups;
   int bn = g.n <= 128 || groups * ((g.n + 255) / 256) < di.sms ? 128 : 256;
   if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
-  // tensor-core scales: pairs from 1024 rows on (SwiGLU backward: 32768 x 7168 x 2048 over 64
-  // groups 565 us single against 588 in pairs, 98304 x 2880 x 5760 over 32 groups 3.33 against 2.19 ms)
+  // tensor-core scales: pairs from 1024 rows on (SwiGLU backward: 32768 x 7168 x 2048 over 64 groups 561 us single against
+  // 590 in pairs, 98304 x 2880 x 5760 over 32 groups 2.31 against 2.13 ms)
   const int mx_cg = getenv("MGF_CTA_GROUP") != nullptr ? cg : (g.total_rows / g.num_groups >= 1024 ? 2 : 1);
   if (bn == 128) cg = 1;
   p.n_tiles = static_cast<int>((g.n + bn - 1) / bn);

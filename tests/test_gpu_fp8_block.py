@@ -8,8 +8,8 @@ multiply-add per block) once per block.  So |acc - exact| <= (256 + 1 + blocks) 
 magnitudes of all products.  Where the tensor core applies the scales (powers of two: exact) it also sums all
 k products: 2 k u S.  bf16 output: 2^-8 of the value.  SwiGLU and its backward are computed from
 bf16 (exactly known) or fp32 inputs in fp32: a few u times their condition, below 64 u of the terms'
-magnitudes, times the output rounding.  The sigmoid is 1 / (1 + e^-z) by the fast division, which gives 0 where
-the denominator is over 2^126: an absolute error of up to 2^-126, times the other factors.
+magnitudes, times the output rounding.  The sigmoid is 1 / (1 + e^-z) by an approximate reciprocal that gives 0
+where the denominator is over 2^126: an absolute error of up to 2^-126, times the other factors.
 """
 
 from __future__ import annotations
