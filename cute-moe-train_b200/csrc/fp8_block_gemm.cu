@@ -5,13 +5,18 @@
 //   MGF_EPI_SWIGLU      aux = bf16(acc + bias[e]), D2 = clamped SwiGLU(aux)
 //   MGF_EPI_SWIGLU_BWD  D = SwiGLU_bwd(acc, aux)
 //
-// The scales change every 128 elements of k, so the tensor cores cannot keep one accumulator over the whole
-// contraction: each block's product goes into one of two TMEM buffers (4 tcgen05.mma of K = 32), and the
-// epilogue warps add it, scaled, to fp32 accumulators in registers while the next block is multiplied into
-// the other buffer.  A thread owns one row and 128 columns (one scale block) of the 128 x 256 tile, so the
-// factor sa * sb is one scalar per thread and block and the promotion is one FMA per element.  The two
-// sides balance: a block's MMAs take 512 clocks at the e4m3 rate, reading 128 x 256 fp32 from TMEM and adding
-// them 256 of the 512.
+// Two forms, chosen on the device by what the scales are (pack_scales_kernel):
+//
+//   gemm_kernel   any fp32 scales.  They change every 128 elements of k, so the tensor cores cannot keep one accumulator over
+//                 the whole contraction: each block's product goes into a TMEM buffer (4 tcgen05.mma of K = 32), and the
+//                 epilogue warps add it, scaled, to fp32 accumulators in registers while the next block is multiplied into
+//                 another buffer.  A thread owns one row and 128 columns (one scale block) of the 128 x 256 tile, so the
+//                 factor sa * sb is one scalar per thread and block and the promotion one FMA per element.  Bound by the
+//                 buffers' way round (about 1200 clocks a block against 512 of its MMAs): 1.60 PFLOP/s at 16384 rows in 4
+//                 groups, n = 5760, k = 2880.  Few rows: the weights' bytes (128 rows over 256 experts, n = 4096,
+//                 k = 7168: 240 us, 6.5 TB/s).
+//   mx_kernel     powers of two.  The tensor cores apply the scales and the accumulator stays in TMEM: 2.1 PFLOP/s at the
+//                 same sizes, bound by shared-memory traffic (operands written and read) and, sustained, by the power cap.
 //
 // B is read as stored, [E, k, n] with unit stride along n (the weights' own layout: MN-major operand) or along
 // k (the transposed view, the input gradient), so one set of codes serves both.  Warp roles, CTA pairs,
