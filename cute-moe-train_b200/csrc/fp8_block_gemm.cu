@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    if (ptx::elect_one()) {
       uint32_t stage = 0, phase = 0;
       uint32_t issued = 0, issued_parity = 0;  // one bit per stage
       bool ok = true;
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t a_kstep = 32u >> 4;
     uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, the TMEM buffers in turn
     bool ok = true, issued_any = false;
-    if (leader && lane == 0) {
+    if (leader && ptx::elect_one()) {
       for (int t = unit; ok && t < total_tiles; t += num_units) {
         for (int kb = 0; kb < nk; ++kb, ++part) {
           const uint32_t buf = part % BUFS, bph = (part / BUFS) & 1;
@@ -699,7 +699,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSetupRegs));
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
+    if (ptx::elect_one()) {
       uint32_t stage = 0, phase = 0;
       uint32_t issued = 0, issued_parity = 0;  // one bit per stage
       bool ok = true;
@@ -745,7 +745,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (one thread of the even CTA)
-    if (leader && lane == 0) {
+    if (leader && ptx::elect_one()) {
       constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
       constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
       constexpr uint32_t a_kstep = 32u >> 4;
@@ -1091,7 +1091,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   int cg = g.total_rows / g.num_groups >= 512 ? 2 : 1;
   if (const char* env = getenv("MGF_CTA_GROUP"); env != nullptr && (env[0] == '1' || env[0] == '2')) cg = env[0] - '0';
   const int64_t groups = g.total_rows < g.num_groups ? g.total_rows : g.num_groups;
-  int bn = g.n <= 128 || groups * ((g.n + 255) / 256) < di.sms ? 128 : 256;
+  int bn = g.n <= 128 || (groups + g.total_rows / BM) * ((g.n + 255) / 256) < di.sms ? 128 : 256;
   if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
   // tensor-core scales: pairs from 1024 rows on (SwiGLU backward: 32768 x 7168 x 2048 over 64 groups 561 us single against
   // 590 in pairs, 98304 x 2880 x 5760 over 32 groups 2.31 against 2.13 ms)

@@ -50,6 +50,17 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// True for one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t yes;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(yes));
+  return yes != 0;
+}
+
 // ---------------------------------------------------------------- TMA
 // 32-byte read-only global load (one whole sector per thread), not allocated in L1.
 __device__ __forceinline__ void ld_nc_v8_noalloc(const void* ptr, uint4& lo, uint4& hi) {
