@@ -12,11 +12,11 @@
 //                 epilogue warps add it, scaled, to fp32 accumulators in registers while the next block is multiplied into
 //                 another buffer.  A thread owns one row and 128 columns (one scale block) of the 128 x 256 tile, so the
 //                 factor sa * sb is one scalar per thread and block and the promotion one FMA per element.  Bound by the
-//                 buffers' way round (about 1200 clocks a block against 512 of its MMAs): 1.60 PFLOP/s at 16384 rows in 4
-//                 groups, n = 5760, k = 2880.  Few rows: the weights' bytes (128 rows over 256 experts, n = 4096,
-//                 k = 7168: 240 us, 6.5 TB/s).
-//   mx_kernel     powers of two.  The tensor cores apply the scales and the accumulator stays in TMEM: 2.1 PFLOP/s at the
-//                 same sizes, bound by shared-memory traffic (operands written and read) and, sustained, by the power cap.
+//                 buffers' way round (about 1000 clocks a block against 512 of its MMAs): 1.7 PFLOP/s at 16384 rows in 4
+//                 groups, n = 5760, k = 2880.  Few rows: the weights' bytes.
+//   mx_kernel     powers of two.  The tensor cores apply the scales and the accumulator stays in TMEM: 2.3 PFLOP/s at the
+//                 same sizes, bound by the products' issue and shared-memory traffic (operands written and read) and,
+//                 sustained, by the power cap.  128 rows over 256 experts, n = 4096, k = 7168: 250 us, 5.9 TB/s of weights.
 //
 // B is read as stored, [E, k, n] with unit stride along n (the weights' own layout: MN-major operand) or along
 // k (the transposed view, the input gradient), so one set of codes serves both.  Warp roles, CTA pairs,
@@ -25,6 +25,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cstdint>
 #include <cstdio>
@@ -424,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ UMMA issuer (one thread of the even CTA)
+    // ------------------------------------------------------------ UMMA issuer (one elected thread of the even CTA)
     constexpr uint32_t idesc = ptx::make_idesc_e4m3(BM * CG, BN, false, B_MN);
     // MN-major B: 128-column chunks of 128 k rows, 16 KB apart, 32 k rows of 128 bytes per instruction;
     // K-major: 32 bytes of every 128-byte row per instruction
@@ -744,7 +745,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
       }
     }
   } else if (warp == 1) {
-    // ------------------------------------------------------------ UMMA issuer (one thread of the even CTA)
+    // ------------------------------------------------------------ UMMA issuer (one elected thread of the even CTA)
     if (leader && ptx::elect_one()) {
       constexpr uint32_t b_lbo = B_MN ? 16384u : 16u;
       constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
@@ -997,12 +998,21 @@ MxSpace mx_space(const mgf_block_gemm_desc& g) {
   return s;
 }
 
-// The tensor cores' scales save the promotion but cost two small launches (packing 5-10 us, the form that returns at
-// once 2.5 us).  From 1024 rows on (n = 5760, k = 2880, 32 groups, SwiGLU: 111 against 114 us at 1024 rows, 143 against 158
-// at 4096; at 256 rows 96 against 98, at 32 rows 70 against 59).  MGF_BLOCK_MX=0|1 forces a choice.
-bool use_mx(const mgf_block_gemm_desc& g) {
+// Tiles of 128 x 256, at most.
+int64_t wide_tiles(const mgf_block_gemm_desc& g) {
+  return (std::min<int64_t>(g.total_rows, g.num_groups) + g.total_rows / BM) * ((g.n + 255) / 256);
+}
+
+// The tensor cores' scales save the promotion but cost two small launches (packing 3-5 us, the form that returns at once
+// 2.5), so they have to be earned in blocks of k per SM: from 24 on with many rows, where the promotion is what a block
+// waits for (8 groups, k = n = 2048: 25 against 19 us at 1024 rows and 14 blocks, 33 against 43 at 4096 rows and 35);
+// from 120 on with few, where both forms wait for the weights and this one keeps more of them under way (128 rows,
+// k = 2880, n = 5760: 32 groups and 118 blocks 82 against 81, 128 groups and 460 blocks 126 against 137; 256 groups,
+// k = 2048, n = 7168: 127 against 136).  MGF_BLOCK_MX=0|1 forces a choice.
+bool use_mx(const mgf_block_gemm_desc& g, int sms) {
   if (const char* env = getenv("MGF_BLOCK_MX"); env != nullptr && (env[0] == '0' || env[0] == '1')) return env[0] == '1';
-  return g.n > 128 && g.total_rows >= 1024;
+  const int64_t blocks = wide_tiles(g) * ((g.k + BK - 1) / BK);
+  return g.n > 128 && blocks >= (g.total_rows >= 1024 ? 24ll : 120ll) * sms;
 }
 
 bool aligned(const void* ptr, unsigned n) { return (reinterpret_cast<uintptr_t>(ptr) & (n - 1u)) == 0; }
@@ -1015,7 +1025,9 @@ extern "C" size_t mgf_block_gemm_desc_size(void) { return sizeof(mgf_block_gemm_
 extern "C" int64_t mgf_block_gemm_workspace_bytes(const mgf_block_gemm_desc* desc) {
   using namespace mgf::block_gemm;
   if (desc == nullptr || desc->num_groups < 1 || desc->total_rows <= 0 || desc->n <= 0 || desc->k <= 0) return 0;
-  return use_mx(*desc) ? mx_space(*desc).bytes() : 0;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  return use_mx(*desc, mgf::device_info(dev).sms) ? mx_space(*desc).bytes() : 0;
 }
 
 extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stream) {
@@ -1082,19 +1094,18 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
     p.stall_test = (env != nullptr && env[0] == '1') ? 1 : 0;
   }
 
-  // Pairs (256-row tiles, half the B bytes per SM) for groups of 512 rows and more on average, as in
-  // moe_gemm_sm100.cu; MGF_CTA_GROUP=1|2 forces.  128-column tiles where one covers n, and where 256-column tiles of
-  // the groups that can have rows would leave SMs without one (4 rows, n = 5760, k = 2880: 16.2 against 18.9 us);
-  // with more tiles the wide ones read fewer bytes of A per product (32 rows: 59.0 against 60.2 us, 256 rows: 97.5
-  // against 107).  MGF_BN=128|256 forces.
+  // Pairs (256-row tiles, half the B bytes per SM) for groups of 2048 rows and more on average (32 groups, k = 2880,
+  // n = 5760, SwiGLU: 1024 rows each 692 single against 739 us in pairs, 3072 rows each 2103 against 2034);
+  // MGF_CTA_GROUP=1|2 forces.  128-column tiles where one covers n, and where 256-column tiles would leave SMs
+  // without one (4 rows, n = 5760, k = 2880: 12.4 against 16 us); with more tiles the wide ones read fewer bytes of A
+  // per product (256 rows: 97.5 against 107 us).  MGF_BN=128|256 forces.
   const bool b_mn = g.b_mn_major != 0;
-  int cg = g.total_rows / g.num_groups >= 512 ? 2 : 1;
+  int cg = g.total_rows / g.num_groups >= 2048 ? 2 : 1;
   if (const char* env = getenv("MGF_CTA_GROUP"); env != nullptr && (env[0] == '1' || env[0] == '2')) cg = env[0] - '0';
-  const int64_t groups = g.total_rows < g.num_groups ? g.total_rows : g.num_groups;
-  int bn = g.n <= 128 || (groups + g.total_rows / BM) * ((g.n + 255) / 256) < di.sms ? 128 : 256;
+  int bn = g.n <= 128 || wide_tiles(g) < di.sms ? 128 : 256;
   if (const char* env = getenv("MGF_BN"); env != nullptr && (atoi(env) == 128 || atoi(env) == 256)) bn = atoi(env);
-  // tensor-core scales: pairs from 1024 rows on (SwiGLU backward: 32768 x 7168 x 2048 over 64 groups 561 us single against
-  // 590 in pairs, 98304 x 2880 x 5760 over 32 groups 2.31 against 2.13 ms)
+  // tensor-core scales: pairs from 1024 rows on (SwiGLU, 32 groups, k = 2880, n = 5760: 512 rows each 306 us
+  // single against 323 in pairs, 2048 rows each 1122 against 1015)
   const int mx_cg = getenv("MGF_CTA_GROUP") != nullptr ? cg : (g.total_rows / g.num_groups >= 1024 ? 2 : 1);
   if (bn == 128) cg = 1;
   p.n_tiles = static_cast<int>((g.n + bn - 1) / bn);
@@ -1120,7 +1131,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   int sms = di.sms - (g.sm_carveout > 0 ? g.sm_carveout : 0);
   if (sms < cg) sms = cg;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (use_mx(g) && g.workspace != nullptr) {
+  if (use_mx(g, di.sms) && g.workspace != nullptr) {
     if (!aligned(g.workspace, 16)) return MGF_ERR_ALIGNMENT;
     const MxSpace sp = mx_space(g);
     uint32_t* ws = static_cast<uint32_t*>(g.workspace);

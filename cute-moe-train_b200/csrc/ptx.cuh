@@ -50,7 +50,9 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
-// True for one lane of a converged warp.
+// True for one lane of a converged warp.  Where it guards tensor and TMA instructions, the compiler knows that one lane is
+// left and keeps their operands in uniform registers; under `lane == 0` it moves each one there first (four
+// products and two commits: 390 against 270 clocks to issue).
 __device__ __forceinline__ bool elect_one() {
   uint32_t yes;
   asm volatile(
