@@ -1095,7 +1095,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   }
 
   // Pairs (256-row tiles, half the B bytes per SM) for groups of 2048 rows and more on average (32 groups, k = 2880,
-  // n = 5760, SwiGLU: 1024 rows each 692 single against 739 us in pairs, 3072 rows each 2103 against 2034);
+  // n = 5760, SwiGLU: 32768 rows 692 single against 739 us in pairs, 98304 rows 2103 against 2034);
   // MGF_CTA_GROUP=1|2 forces.  128-column tiles where one covers n, and where 256-column tiles would leave SMs
   // without one (4 rows, n = 5760, k = 2880: 12.4 against 16 us); with more tiles the wide ones read fewer bytes of A
   // per product (256 rows: 97.5 against 107 us).  MGF_BN=128|256 forces.

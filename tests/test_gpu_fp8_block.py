@@ -445,3 +445,27 @@ def test_two_streams_and_a_captured_launch_with_new_scales(monkeypatch):
         xb.copy_(scales[1])
         graph.replay()
         assert torch.equal(out, want[i])
+
+
+@pytest.mark.parametrize("powers", [False, True])
+def test_few_rows_over_much_weight(powers, monkeypatch):
+    """Few rows, but so many blocks of weights that the launcher itself offers them to the form with the scales in the
+    tensor cores; which form runs is the scales' matter."""
+    import cutlass_op.bf16_grouped_mm as m
+    from cutlass_op.bf16_grouped_mm import fp8_block
+
+    for name in ("MGF_BLOCK_MX", "MGF_CTA_GROUP", "MGF_BN"):
+        monkeypatch.delenv(name, raising=False)
+    K, N = 2200, 4200
+    counts = [1, 0, 5, 40, 2, 33] + [1] * 64
+    a, b, offs, sa, sb, bias = _case(len(counts), K, N, counts, "kn", 11, extra_rows=2)
+    if powers:
+        for t in (sa, sb):
+            t.copy_(torch.exp2(torch.randint(-6, 7, t.shape, generator=_gen(8), device="cuda").float()))
+    acc, mag = _exact(a, b, offs, sa, sb)
+    biased = acc + bias.double()[_row_of(offs, acc.shape[0])]
+    rows = int(offs[-1])
+    tol = (2 * K if powers else 257 + sa.shape[1]) * U * mag + U * biased.abs() + 2.0 ** -8 * biased.abs()
+    out = fp8_block.grouped_mm_fp8_block(a, b, offs, sa, sb, bias)
+    _within("out", out[:rows], biased[:rows], tol[:rows])
+    m.check_device_status()
