@@ -58,6 +58,18 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
+// min and max that keep a NaN, as the formula's clamps do (fminf and fmaxf give the other operand).
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float y;
+  asm("min.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+
 // sigma(z) = 0.5 * tanh(z / 2) + 0.5, the form the reference's SwiGLU visitors use
 // (csrc/grouped_mm_swiglu_visitor.cuh:309-334, csrc/grouped_mm_swiglu_bwd_visitor.cuh:35-68), on the
 // hardware tanh approximation (one MUFU operation; max relative error about 2^-11, below bf16's 2^-8).

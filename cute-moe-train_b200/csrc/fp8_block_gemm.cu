@@ -215,13 +215,14 @@ __device__ __forceinline__ float sigmoid(float gate, float neg_alpha_log2e) {
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ float swiglu(float g, float u, float neg_alpha_log2e, float limit) {
-  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
+  const float gc = min_nan(g, limit), uc = max_nan(min_nan(u, limit), -limit);
   return gc * sigmoid(gc, neg_alpha_log2e) * (uc + 1.0f);
 }
-// d_gate = gs (uc + 1) sig (1 + alpha gc (1 - sig)), d_up = gs gc sig, each 0 where its input is clamped.
+// d_gate = gs (uc + 1) sig (1 + alpha gc (1 - sig)), d_up = gs gc sig, each 0 where its own input is clamped or NaN (the
+// clamp's derivative is 1 in its range only); a NaN of the other input or of gs stays one.
 __device__ __forceinline__ uint32_t swiglu_bwd(float gs, uint32_t aux_word, float alpha, float neg_alpha_log2e, float limit) {
   const float g = bf16_lo(aux_word), u = bf16_hi(aux_word);
-  const float gc = fminf(g, limit), uc = fmaxf(fminf(u, limit), -limit);
+  const float gc = min_nan(g, limit), uc = max_nan(min_nan(u, limit), -limit);
   const float sig = sigmoid(gc, neg_alpha_log2e), t = gs * sig;
   const float d_gate = g <= limit ? t * (uc + 1.0f) * fmaf(alpha * gc, 1.0f - sig, 1.0f) : 0.0f;
   const float d_up = fabsf(u) <= limit ? t * gc : 0.0f;
