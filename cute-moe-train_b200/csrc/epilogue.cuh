@@ -82,17 +82,18 @@ __device__ __forceinline__ float sigmoidf_fast(float z) { return fmaf(0.5f, tanh
 
 // SwiGLU forward on one (gate, up) pair of bf16-rounded values.
 __device__ __forceinline__ float swiglu_fwd(float g, float u, float alpha, float limit) {
-  const float gc = fminf(g, limit);
-  const float uc = fmaxf(fminf(u, limit), -limit);
+  const float gc = min_nan(g, limit);
+  const float uc = max_nan(min_nan(u, limit), -limit);
   return gc * sigmoidf_fast(alpha * gc) * (uc + 1.0f);
 }
 
-// SwiGLU backward for one packed (gate, up) word of aux; returns packed (d_gate, d_up).
+// SwiGLU backward for one packed (gate, up) word of aux; returns packed (d_gate, d_up), each 0 where its own input is
+// clamped or NaN; a NaN of the other input or of gs stays one.
 __device__ __forceinline__ uint32_t swiglu_bwd_word(float gs, uint32_t aux_word, float alpha, float limit) {
   const float g = bf16_lo(aux_word);
   const float u = bf16_hi(aux_word);
-  const float gc = fminf(g, limit);
-  const float uc = fmaxf(fminf(u, limit), -limit);
+  const float gc = min_nan(g, limit);
+  const float uc = max_nan(min_nan(u, limit), -limit);
   const float sig = sigmoidf_fast(alpha * gc);
   float d_gate = gs * (uc + 1.0f) * sig * (1.0f + alpha * gc * (1.0f - sig));
   float d_up = gs * gc * sig;

@@ -133,3 +133,87 @@ def _moe_ffn_keeps_nan(precision):
     _same_but_for_nan(moe_ffn(bad, logits, 2, *w, precision=precision), clean, nan)
     leaf = bad.clone().requires_grad_(True)
     _same_but_for_nan(moe_ffn(leaf, logits, 2, *w, precision=precision).detach(), clean, nan)
+
+
+# ------------------------------------------------------------------------------------------------ bf16, e4m3 with row scales
+def test_bf16_moe_ffn_keeps_the_nan_of_a_token():
+    _moe_ffn_keeps_nan("bf16")
+
+
+@pytest.mark.parametrize("rows,cg", [(150, "1"), (150, "2")])
+@pytest.mark.parametrize("store_aux", [True, False])
+def test_bf16_swiglu_keeps_nan(rows, cg, store_aux, monkeypatch):
+    from cutlass_op.bf16_grouped_mm import grouped_mm_swiglu
+
+    monkeypatch.setenv("MGF_CTA_GROUP", cg)
+    g = _gen(4)
+    E, K, N = 2, 320, 272
+    x = _randn(g, rows, K).to(torch.bfloat16)
+    w = (_randn(g, E, K, N) / math.sqrt(K)).to(torch.bfloat16)
+    bias = (0.1 * _randn(g, E, N)).to(torch.bfloat16)
+    offs = torch.tensor([70, rows], dtype=torch.int32, device="cuda")
+
+    def f(x, bias):
+        if store_aux:
+            return grouped_mm_swiglu(x, w, offs, bias)[0]
+        return torch.ops.grouped_mm.mm_swiglu_noaux(x, w, offs, bias, ALPHA, LIMIT)
+
+    s0 = f(x, bias)
+    assert not s0.isnan().any()
+    bad = x.clone()
+    bad[7, 300] = math.nan
+    nan = torch.zeros(rows, N // 2, dtype=torch.bool, device="cuda")
+    nan[7] = True
+    _same_but_for_nan(f(bad, bias), s0, nan)
+    b = bias.clone()
+    b[0, 6], b[1, 9] = math.nan, math.nan
+    nan = torch.zeros(rows, N // 2, dtype=torch.bool, device="cuda")
+    nan[:70, 3], nan[70:, 4] = True, True
+    _same_but_for_nan(f(x, b), s0, nan)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("cg", ["1", "2"])
+def test_swiglu_backward_keeps_nan(cg, e4m3, monkeypatch):
+    from cutlass_op.bf16_grouped_mm import fp8
+
+    monkeypatch.setenv("MGF_CTA_GROUP", cg)
+    g = _gen(5)
+    E, K, I, rows = 2, 320, 272, 150
+    grad = _randn(g, rows, K).to(torch.bfloat16)
+    w = (_randn(g, E, K, I) / math.sqrt(K)).to(torch.bfloat16)
+    aux = (4 * _randn(g, rows, 2 * I)).to(torch.bfloat16)
+    offs = torch.tensor([70, rows], dtype=torch.int32, device="cuda")
+    if e4m3:
+        (qg, sg), (qw, sw) = fp8.quantize_rows(grad), fp8.quantize_weights(w)
+
+        def f(aux):
+            return fp8.grouped_mm_swiglu_bwd_fp8(qg, qw, offs, aux, sg, sw, ALPHA, LIMIT)
+    else:
+        def f(aux):
+            return torch.ops.grouped_mm.mm_swiglu_bwd(grad, w, offs, aux, ALPHA, LIMIT)
+    clean = f(aux)
+    assert not clean.isnan().any()
+    gate, up = aux[:, 0::2].float(), aux[:, 1::2].float()
+    bad, ng, nu = _spoilt(aux)
+    want = clean.clone()
+    want[:, 0::2][ng], want[:, 1::2][nu] = 0.0, 0.0
+    nan = _pairs(nu & (gate <= LIMIT) & ~ng, ng & (up.abs() <= LIMIT) & ~nu)
+    _same_but_for_nan(f(bad), want, nan)
+
+
+def test_e4m3_row_scaled_swiglu_keeps_nan():
+    from cutlass_op.bf16_grouped_mm import fp8
+
+    g = _gen(6)
+    E, K, N, rows = 2, 320, 272, 150
+    x = _randn(g, rows, K).to(torch.bfloat16)
+    w = (_randn(g, E, K, N) / math.sqrt(K)).to(torch.bfloat16)
+    bias = (0.1 * _randn(g, E, N)).to(torch.bfloat16)
+    offs = torch.tensor([70, rows], dtype=torch.int32, device="cuda")
+    (qx, sx), (qw, sw) = fp8.quantize_rows(x), fp8.quantize_weights(w)
+    s0, _ = fp8.grouped_mm_swiglu_fp8(qx, qw, offs, sx, sw, bias, ALPHA, LIMIT)
+    bias[1, 8] = math.nan
+    nan = torch.zeros(rows, N // 2, dtype=torch.bool, device="cuda")
+    nan[70:, 4] = True
+    _same_but_for_nan(fp8.grouped_mm_swiglu_fp8(qx, qw, offs, sx, sw, bias, ALPHA, LIMIT)[0], s0, nan)
