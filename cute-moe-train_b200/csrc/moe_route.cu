@@ -1,6 +1,7 @@
 // Router of the MoE block: top-k experts of every token and their weights, and the logits' gradient.
 //
-//   key_e = l_e (+ bias_e, fp32)                     selection only; ties go to the lowest expert
+//   key_e = l_e (+ bias_e, fp32)                     selection only; ties go to the lowest expert.  A bias that
+//           balances the load by the scores (BIAS_ON_SCORE): key_e = s(l_e) + bias_e or softmax_e(l) + bias_e
 //   chosen = the topk largest keys; a key of -inf is never chosen (id -1, weight 0), NaN sorts first
 //   softmax:  w_j = scale * exp(l_j - m) / sum exp(l_i - m), the sum over the chosen experts
 //             (renormalize) or over all experts
@@ -67,6 +68,11 @@ __device__ __forceinline__ float log_score(float v, int score) {
   return score == MGF_ROUTE_SIGMOID ? fminf(v, 0.0f) - log1pf(expf(-fabsf(v))) : v;
 }
 
+// The score itself; row_max and row_sum: of the softmax over all experts.
+__device__ __forceinline__ float score_of(float v, int score, float row_max, float row_sum) {
+  return score == MGF_ROUTE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : expf(v - row_max) / row_sum;
+}
+
 // p_j of the chosen logits, one per lane (0 where `live` is false).
 __device__ __forceinline__ float chosen_prob(float v, bool live, int score, bool renorm, float row_max, float row_sum) {
   if (renorm) {
@@ -76,14 +82,13 @@ __device__ __forceinline__ float chosen_prob(float v, bool live, int score, bool
     const float s = warp_sum(p);
     return live ? p / s : 0.0f;
   }
-  if (!live) return 0.0f;
-  return score == MGF_ROUTE_SIGMOID ? 1.0f / (1.0f + expf(-v)) : expf(v - row_max) / row_sum;
+  return live ? score_of(v, score, row_max, row_sum) : 0.0f;
 }
 
 template <typename T, int R, bool PACKED>
 __global__ void __launch_bounds__(32 * kWarpsPerBlock)
     route_kernel(const T* __restrict__ logits, int64_t ld, int64_t tokens, int E, int topk, int score, bool renorm,
-                 float scale, const float* __restrict__ bias, const uint8_t* __restrict__ token_mask,
+                 float scale, const float* __restrict__ bias, bool on_score, const uint8_t* __restrict__ token_mask,
                  float* __restrict__ weights, int64_t* __restrict__ idx) {
   const int lane = threadIdx.x & 31;
   const int64_t t = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) >> 5;
@@ -107,7 +112,7 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
       // the low half of a bf16 key says nothing; the earlier expert gets the larger word
       if (PACKED && key[i] != 0u) key[i] = (key[i] & 0xffff0000u) | static_cast<uint32_t>(0xffff - e);
     }
-    if (score == MGF_ROUTE_SOFTMAX && !renorm) {
+    if (score == MGF_ROUTE_SOFTMAX && (!renorm || on_score)) {
       float m = v[0], s = 0.0f;
 #pragma unroll
       for (int i = 1; i < R; ++i) m = fmaxf(m, v[i]);
@@ -115,6 +120,13 @@ __global__ void __launch_bounds__(32 * kWarpsPerBlock)
 #pragma unroll
       for (int i = 0; i < R; ++i) s += (lane + 32 * i < E) ? expf(v[i] - row_max) : 0.0f;
       row_sum = warp_sum(s);
+    }
+    if (on_score) {  // there is a bias
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int e = lane + 32 * i;
+        if (e < E && v[i] != -INFINITY) key[i] = order_key(score_of(v[i], score, row_max, row_sum) + __ldg(bias + e));
+      }
     }
     for (int j = 0; j < topk; ++j) {
       uint32_t best = key[0];
@@ -235,6 +247,8 @@ extern "C" int mgf_moe_route(const void* logits, int32_t dtype, int64_t ld, int6
                              int32_t topk, int32_t score, int32_t renormalize, float scale, const float* bias,
                              const uint8_t* token_mask, float* weights, int64_t* expert_idx, void* stream) {
   using namespace mgf;
+  const bool on_score = (score & MGF_ROUTE_BIAS_ON_SCORE) != 0 && bias != nullptr;
+  score &= ~MGF_ROUTE_BIAS_ON_SCORE;
   if (!route_args_ok(dtype, tokens, num_experts, topk, score)) return MGF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return MGF_OK;
   if (logits == nullptr || weights == nullptr || expert_idx == nullptr) return MGF_ERR_INVALID_ARGUMENT;
@@ -247,7 +261,7 @@ extern "C" int mgf_moe_route(const void* logits, int32_t dtype, int64_t ld, int6
       auto kern = kBf16 && bias == nullptr ? route_kernel<T, R, kBf16> : route_kernel<T, R, false>;
       kern<<<grid, 32 * kWarpsPerBlock, 0, static_cast<cudaStream_t>(stream)>>>(
           static_cast<const T*>(logits), ld, tokens, num_experts, topk, score, renormalize != 0, scale, bias,
-          token_mask, weights, expert_idx);
+          on_score, token_mask, weights, expert_idx);
       return cudaGetLastError() == cudaSuccess ? MGF_OK : MGF_ERR_CUDA;
     });
   };
@@ -261,6 +275,7 @@ extern "C" int mgf_moe_route_bwd(const void* logits, int32_t dtype, int64_t ld, 
                                  const int64_t* expert_idx, const float* grad_weights, void* grad_logits, int64_t ldg,
                                  void* stream) {
   using namespace mgf;
+  score &= ~MGF_ROUTE_BIAS_ON_SCORE;  // the bias is not in the weights
   if (!route_args_ok(dtype, tokens, num_experts, topk, score)) return MGF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return MGF_OK;
   if (logits == nullptr || expert_idx == nullptr || grad_weights == nullptr || grad_logits == nullptr)

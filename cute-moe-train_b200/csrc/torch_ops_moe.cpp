@@ -59,7 +59,8 @@ int32_t check_route(const Tensor& logits, int64_t topk, int64_t score) {
   const int64_t E = logits.size(1);
   TORCH_CHECK(E >= 1 && E <= 1024, "moe_route: the number of experts must be in [1, 1024], got ", E);
   TORCH_CHECK(topk >= 1 && topk <= std::min<int64_t>(E, 32), "moe_route: topk must be in [1, min(E, 32)], got ", topk);
-  TORCH_CHECK(score == MGF_ROUTE_SOFTMAX || score == MGF_ROUTE_SIGMOID, "moe_route: unknown score");
+  const int64_t kind = score & ~int64_t{MGF_ROUTE_BIAS_ON_SCORE};
+  TORCH_CHECK(kind == MGF_ROUTE_SOFTMAX || kind == MGF_ROUTE_SIGMOID, "moe_route: unknown score");
   return dtype_code(logits, "moe_route");
 }
 

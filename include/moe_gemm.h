@@ -253,12 +253,15 @@ int mgf_fp8_quantize_weights_both(const void* w, int64_t E, int64_t K, int64_t N
  * (no counterpart in the reference, whose path starts from rows already in expert order). */
 enum mgf_dtype { MGF_DT_BF16 = 0, MGF_DT_F16 = 1, MGF_DT_F32 = 2 };
 enum mgf_route_score { MGF_ROUTE_SOFTMAX = 0, MGF_ROUTE_SIGMOID = 1 };
+#define MGF_ROUTE_BIAS_ON_SCORE 0x100 /* or'ed to a score: the bias is added to the score, not to the logit */
 
 /* Router.  logits [tokens, E] (E <= 1024, topk <= min(E, 32), row stride ld): the topk experts with the
- * largest logit + bias (bias fp32 [E] or NULL, selection only), largest first, ties to the lowest expert.
+ * largest logit + bias (bias fp32 [E] or NULL, selection only), largest first, ties to the lowest expert.  With
+ * MGF_ROUTE_BIAS_ON_SCORE it is the largest score + bias instead, the score being the sigmoid or the softmax over
+ * all experts in fp32 (the order differs: neither is linear); without a bias the flag changes nothing.
  * weights fp32 [tokens, topk]: scale * softmax (over the chosen experts if renormalize, else over all) or
  * scale * sigmoid (divided by the chosen experts' sum if renormalize) of the logits without bias.
- * expert_idx int64 [tokens, topk].  A logit or logit + bias of -inf is never chosen: slots left over, and
+ * expert_idx int64 [tokens, topk].  A logit of -inf is never chosen, nor is a sum with the bias of -inf: slots left over, and
  * all slots of tokens whose token_mask (bytes, or NULL) is 0, get id -1 and weight 0.
  * mgf_moe_route_bwd: grad_logits [tokens, E] (row stride ldg, every element written) from the gradient of
  * the weights; the chosen experts are those of expert_idx. */
