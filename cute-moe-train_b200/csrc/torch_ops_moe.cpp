@@ -498,6 +498,11 @@ std::tuple<Tensor, Tensor> call_unpermute_bwd(const Tensor& g, const Tensor& row
   return h.call(g, rows, offs, row_of_copy, weights, need_rows, need_weights);
 }
 
+// Forward-mode derivatives are refused, not dropped: a dual tensor need not require grad, so it would go below autograd.
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, ": forward-mode derivatives are not implemented");
+}
+
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
 // A gradient as the kernels take it: unit stride along the last dimension, rows apart.
@@ -597,6 +602,7 @@ struct Unpermute : torch::autograd::Function<Unpermute> {
 std::tuple<Tensor, Tensor> moe_route_autograd(const Tensor& logits, int64_t topk, int64_t score, bool renormalize,
                                               double scale, const std::optional<Tensor>& bias,
                                               const std::optional<Tensor>& mask) {
+  no_tangent(logits, "moe_route");
   if (!wants_grad(logits)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_route(logits, topk, score, renormalize, scale, bias, mask);
@@ -605,6 +611,7 @@ std::tuple<Tensor, Tensor> moe_route_autograd(const Tensor& logits, int64_t topk
   return {r[0], r[1]};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> moe_permute_autograd(const Tensor& x, const Tensor& idx, int64_t E) {
+  no_tangent(x, "moe_permute");
   if (!wants_grad(x)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_permute(x, idx, E);
@@ -613,6 +620,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> moe_permute_autograd(const Tensor& x,
   return {r[0], r[1], r[2], r[3]};
 }
 Tensor moe_permute_rows_autograd(const Tensor& x, const Tensor& offs, const Tensor& row_of_copy) {
+  no_tangent(x, "moe_permute");
   if (!wants_grad(x)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_permute_rows(x, offs, row_of_copy);
@@ -621,6 +629,8 @@ Tensor moe_permute_rows_autograd(const Tensor& x, const Tensor& offs, const Tens
 }
 Tensor moe_unpermute_autograd(const Tensor& rows, const Tensor& offs, const Tensor& row_of_copy,
                               const std::optional<Tensor>& weights) {
+  no_tangent(rows, "moe_unpermute");
+  if (weights.has_value()) no_tangent(*weights, "moe_unpermute");
   if (!wants_grad(rows) && !(weights.has_value() && wants_grad(*weights))) {
     at::AutoDispatchBelowADInplaceOrView below;
     return call_unpermute(rows, offs, row_of_copy, weights);

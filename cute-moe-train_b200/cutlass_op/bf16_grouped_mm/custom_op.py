@@ -22,6 +22,7 @@ shape inference and autograd with the same contract as Butterfingrz/CuTe-MoE-Tra
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _ext  # noqa: F401  (loads the native libraries and registers the operators)
 from .optimer import timed
@@ -41,6 +42,16 @@ def dtype_to_int(dtype: torch.dtype | None) -> int:
 
 def _dtype_from_int(out_dtype: int) -> torch.dtype | None:
     return None if out_dtype == -1 else _CODE_SCALAR_TYPE[out_dtype]
+
+
+def refuse_tangents(what: str, *tensors: torch.Tensor | None) -> None:
+    """Raise where a tensor carries a forward-mode tangent: the operators have no such derivative, and one that does not
+    require grad as well would pass below their autograd, its tangent lost without a word."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{what}: forward-mode derivatives are not implemented")
 
 
 def _padded(n: int, dtype: torch.dtype) -> int:

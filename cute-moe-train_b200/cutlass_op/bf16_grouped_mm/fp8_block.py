@@ -18,7 +18,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext  # noqa: F401  (registers the operators)
-from .custom_op import _padded
+from .custom_op import _padded, refuse_tangents
 from .optimer import timed
 from .permute import _codes_fake
 
@@ -50,6 +50,7 @@ def quantize_rows_block(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """bf16 [M, K] -> (e4m3 [M, K], fp32 [M, ceil(K / 128)]), both with a 16-byte row pitch:
     x[m, k] ~= q[m, k] * scale[m, k // 128].  Non-finite elements become NaN codes and do not enter their
     block's scale."""
+    refuse_tangents("quantize_rows_block", x)
     with timed("fp8_quantize"):
         return torch.ops.grouped_mm.fp8_quantize_rows_block.default(x.detach())
 
@@ -58,6 +59,7 @@ def quantize_weights_block(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]
     """bf16 [E, K, N] (unit stride along N or along K) -> (e4m3 [E, K, N] in the same layout, fp32
     [E, ceil(K / 128), ceil(N / 128)]): w[e, k, n] ~= q[e, k, n] * scale[e, k // 128, n // 128].
     ``q.transpose(1, 2), scale.transpose(1, 2)`` are the codes of ``w.transpose(1, 2)``."""
+    refuse_tangents("quantize_weights_block", w)
     with timed("fp8_quantize"):
         return torch.ops.grouped_mm.fp8_quantize_weights_block.default(w.detach())
 
@@ -100,6 +102,7 @@ def grouped_mm_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.T
     apart), scale_a fp32 [total_M, ceil(K / 128)], scale_b fp32 [E, ceil(K / 128), ceil(N / 128)] (any strides),
     offs int32 [E] cumulative row ends, N a multiple of 8.  Rows behind offs[-1] are not written.
     """
+    refuse_tangents("grouped_mm_fp8_block", scale_a, scale_b, bias)
     with timed("fp8_block_mm"):
         return torch.ops.grouped_mm.mm_fp8_block.default(mat_a, mat_b, offs, scale_a, scale_b, bias)
 
@@ -109,6 +112,7 @@ def grouped_mm_swiglu_fp8_block(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: 
                                 swiglu_limit: float = 7.0) -> tuple[torch.Tensor, torch.Tensor]:
     """The product + bias + clamped SwiGLU -> (swiglu_out [total_M, I], aux_biased_acc [total_M, 2I]), the
     activation computed from the stored (bf16) aux; mat_b's columns interleave gate and up."""
+    refuse_tangents("grouped_mm_swiglu_fp8_block", scale_a, scale_b, bias)
     with timed("fp8_block_up_swiglu_fwd"):
         return torch.ops.grouped_mm.mm_swiglu_fp8_block.default(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha,
                                                         swiglu_limit)
@@ -119,6 +123,7 @@ def grouped_mm_swiglu_bwd_fp8_block(grad_output: torch.Tensor, down_w_t: torch.T
                                     swiglu_alpha: float = 1.702, swiglu_limit: float = 7.0) -> torch.Tensor:
     """SwiGLU backward of the product grad_output @ down_w_t against aux -> grad_aux bf16 [total_M, 2I]
     (interleaved like aux)."""
+    refuse_tangents("grouped_mm_swiglu_bwd_fp8_block", aux_biased_acc, scale_a, scale_b)
     with timed("fp8_block_down_dgrad_swiglu_bwd"):
         return torch.ops.grouped_mm.mm_swiglu_bwd_fp8_block.default(grad_output, down_w_t, offs, aux_biased_acc, scale_a,
                                                             scale_b, swiglu_alpha, swiglu_limit)

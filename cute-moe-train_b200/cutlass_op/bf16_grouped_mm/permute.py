@@ -20,7 +20,7 @@ from typing import NamedTuple
 import torch
 
 from . import _ext  # noqa: F401  (registers the operators)
-from .custom_op import _padded
+from .custom_op import _padded, refuse_tangents
 from .optimer import timed
 
 
@@ -121,6 +121,7 @@ def moe_permute_fp8(x: torch.Tensor, expert_idx: torch.Tensor | None = None, num
     """``quantize_rows_block`` of the rows of ``moe_permute`` (bf16 x) in one pass over x: (e4m3 codes
     [tokens * topk, hidden], fp32 scales [tokens * topk, ceil(hidden / 128)], plan).  Rows behind offs[-1]
     have zero codes and scales.  No autograd: the codes feed inference, or a backward that uses x."""
+    refuse_tangents("moe_permute_fp8", x)
     with timed("moe_permute_fp8"):
         if plan is not None:
             return (*torch.ops.grouped_mm.moe_permute_rows_fp8.default(x.detach(), plan.offs, plan.row_of_copy), plan)
