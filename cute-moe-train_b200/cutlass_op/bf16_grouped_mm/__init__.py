@@ -32,6 +32,7 @@ def grouped_mm(
     ragged-M case; 2D x 2D is ragged-K (output [E, M, N]); 3D x 3D is a batched GEMM.  ``bias``
     [E, N] is added per group.  ``out_dtype`` must be None or the input dtype (bf16).
     """
+    _custom_op.refuse_tangents("grouped_mm", mat_a, mat_b, bias)
     return torch.ops.grouped_mm.mm(mat_a, mat_b, offs, bias, _custom_op.dtype_to_int(out_dtype))
 
 
@@ -57,6 +58,7 @@ def grouped_mm_swiglu(
         ``aux_biased_acc`` must be handed to :func:`grouped_mm_downproj`, which routes the
         gradient back through it; a gradient reaching ``swiglu_out`` directly raises.
     """
+    _custom_op.refuse_tangents("grouped_mm_swiglu", mat_a, mat_b, bias)
     with timed("up_swiglu_fwd"):
         return torch.ops.grouped_mm.mm_swiglu(mat_a, mat_b, offs, bias, swiglu_alpha, swiglu_limit)
 
@@ -75,6 +77,7 @@ def grouped_mm_downproj(
     Forward equals ``grouped_mm(mat_a, mat_b, offs=offs, bias=bias)``.  Backward computes
     ``grad_aux = SwiGLU_bwd(grad_out @ mat_b^T, aux_biased_acc)`` in one fused launch.
     """
+    _custom_op.refuse_tangents("grouped_mm_downproj", mat_a, mat_b, bias, aux_biased_acc)
     with timed("down_fwd"):
         return torch.ops.grouped_mm.mm_downproj(
             mat_a, mat_b, offs, bias, aux_biased_acc, swiglu_alpha, swiglu_limit

@@ -26,7 +26,7 @@ from __future__ import annotations
 import torch
 
 from . import _ext  # noqa: F401  (registers the operators)
-from .custom_op import _padded
+from .custom_op import _padded, refuse_tangents
 from .optimer import timed
 
 E4M3_MAX = 448.0
@@ -157,6 +157,7 @@ def dequantize_weights(q: torch.Tensor, scale: torch.Tensor) -> torch.Tensor:
 def grouped_mm_fp8(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.Tensor, scale_a: torch.Tensor,
                    scale_b: torch.Tensor, bias: torch.Tensor | None = None) -> torch.Tensor:
     """Ragged-M e4m3 grouped GEMM with row-wise scales (+ per-expert bf16 bias) -> bf16 [total_M, N]."""
+    refuse_tangents("grouped_mm_fp8", scale_a, scale_b, bias)
     with timed("fp8_mm"):
         return torch.ops.grouped_mm.mm_fp8(mat_a, mat_b, offs, scale_a, scale_b, bias)
 
@@ -165,6 +166,7 @@ def grouped_mm_swiglu_fp8(mat_a: torch.Tensor, mat_b: torch.Tensor, offs: torch.
                           scale_b: torch.Tensor, bias: torch.Tensor, swiglu_alpha: float = 1.702,
                           swiglu_limit: float = 7.0) -> tuple[torch.Tensor, torch.Tensor]:
     """e4m3 up-projection + bias + clamped SwiGLU -> (swiglu_out [total_M, I], aux_biased_acc [total_M, 2I])."""
+    refuse_tangents("grouped_mm_swiglu_fp8", scale_a, scale_b, bias)
     with timed("fp8_up_swiglu_fwd"):
         return torch.ops.grouped_mm.mm_swiglu_fp8(mat_a, mat_b, offs, scale_a, scale_b, bias, swiglu_alpha,
                                                   swiglu_limit)
@@ -174,6 +176,7 @@ def grouped_mm_swiglu_bwd_fp8(grad_output: torch.Tensor, down_w_t: torch.Tensor,
                               aux_biased_acc: torch.Tensor, scale_a: torch.Tensor, scale_b: torch.Tensor,
                               swiglu_alpha: float = 1.702, swiglu_limit: float = 7.0) -> torch.Tensor:
     """e4m3 down-proj dgrad + SwiGLU backward -> grad_aux bf16 [total_M, 2I] (interleaved)."""
+    refuse_tangents("grouped_mm_swiglu_bwd_fp8", aux_biased_acc, scale_a, scale_b)
     with timed("fp8_down_dgrad_swiglu_bwd"):
         return torch.ops.grouped_mm.mm_swiglu_bwd_fp8(grad_output, down_w_t, offs, aux_biased_acc, scale_a, scale_b,
                                                       swiglu_alpha, swiglu_limit)

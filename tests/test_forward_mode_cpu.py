@@ -72,3 +72,28 @@ def test_moe_block(precision):
     _refused(lambda t: moe_ffn(_meta(10, 128), t, 2, *w, precision=precision), logits)
     for i, t in enumerate(w):
         _refused(lambda t, i=i: moe_ffn(_meta(10, 128), logits, 2, *w[:i], t, *w[i + 1:], precision=precision), t)
+
+
+def test_bf16_and_row_scaled_products():
+    import cutlass_op.bf16_grouped_mm as m
+    from cutlass_op.bf16_grouped_mm import fp8
+
+    offs = _meta(2, dtype=torch.int32)
+    x, w, b, aux = _meta(10, 128), _meta(2, 128, 256), _meta(2, 256), _meta(10, 512)
+    _refused(lambda t: m.grouped_mm(t, w, offs, b), x)
+    _refused(lambda t: m.grouped_mm(x, t, offs, b), w)
+    _refused(lambda t: m.grouped_mm(x, w, offs, t), b)
+    _refused(lambda t: m.grouped_mm_swiglu(t, w, offs, b)[0], x)
+    _refused(lambda t: m.grouped_mm_swiglu(x, t, offs, b)[0], w)
+    _refused(lambda t: m.grouped_mm_swiglu(x, w, offs, t)[0], b)
+    _refused(lambda t: m.grouped_mm_downproj(t, w, offs, b, aux), x)
+    _refused(lambda t: m.grouped_mm_downproj(x, t, offs, b, aux), w)
+    _refused(lambda t: m.grouped_mm_downproj(x, w, offs, t, aux), b)
+    _refused(lambda t: m.grouped_mm_downproj(x, w, offs, b, t), aux)
+    e4m3, f32 = torch.float8_e4m3fn, torch.float32
+    a = (_meta(10, 128, dtype=e4m3), _meta(2, 256, 128, dtype=e4m3).transpose(1, 2), offs)
+    s = (_meta(10, dtype=f32), _meta(2, 256, dtype=f32))
+    _refused(lambda t: fp8.grouped_mm_fp8(*a, *s, t), b)
+    _refused(lambda t: fp8.grouped_mm_fp8(*a, t, s[1]), s[0])
+    _refused(lambda t: fp8.grouped_mm_swiglu_fp8(*a, *s, t)[0], b)
+    _refused(lambda t: fp8.grouped_mm_swiglu_bwd_fp8(*a, t, *s), aux)
