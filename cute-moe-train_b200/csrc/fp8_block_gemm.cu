@@ -32,6 +32,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "drain.cuh"
 #include "epilogue.cuh"
 #include "host.h"
 #include "moe_gemm.h"
@@ -46,7 +47,6 @@ constexpr int kMaxGroups = 1024;
 constexpr int kNumEpiWarps = 8;     // two warpgroups, each half of the tile's columns
 constexpr int kThreads = 64 + 32 * kNumEpiWarps;
 constexpr uint64_t kWaitLimitNs = 1500ull * 1000ull * 1000ull;  // 1.5 s per pipeline wait
-constexpr uint64_t kDrainLimitNs = 100ull * 1000ull * 1000ull;
 
 template <int BN, int CG>
 struct Cfg {
@@ -64,7 +64,7 @@ struct Cfg {
   // wake-up), which two buffers of 256 columns hide half of and four of 128 columns all of.
   static constexpr int TMEM_COLS = 512;
   static constexpr int BUFS = TMEM_COLS / BN;
-  static_assert(STAGES >= 3 && (2 * STAGES + 2 * BUFS + 1) * 8 + 8 <= BAR_BYTES && SMEM_BYTES <= 227 * 1024, "shared memory");
+  static_assert(STAGES >= 3 && (2 * STAGES + 2 * BUFS + 1) * 8 + 16 <= BAR_BYTES && SMEM_BYTES <= 227 * 1024, "shared memory");
 };
 
 struct Params {
@@ -85,7 +85,7 @@ struct Params {
   int64_t ld_aux;
   float alpha, limit;
   int aux_v8, d_v8, d2_v8;  // base 32-byte aligned and row pitch a multiple of 32 bytes
-  int stall_test;           // test hook: no tile is loaded, so every consumer wait runs out
+  int stall_test;           // test hook: 1: no tile is loaded, 2: none is multiplied; every wait behind that runs out
   unsigned int* status;
   // The form with the scales in the tensor cores (below) runs where every scale is a power of two, the form with
   // the promotion in registers where one is not: pack_scales_kernel leaves one word per block, not 0 where it
@@ -120,9 +120,9 @@ __device__ __forceinline__ void arrive_relaxed_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
-// Wait for phase `parity` of an mbarrier for at most `limit_ns`.
+// Wait for phase `parity` of an mbarrier for at most kWaitLimitNs.
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                             unsigned int* status, uint64_t limit_ns = kWaitLimitNs) {
+                                             unsigned int* status) {
   // The waits come once per block of k, so the common case reads no timer (a %globaltimer read costs far
   // more than the wait): the limit counts from the 64th failed try.
   uint64_t t0 = 0;
@@ -131,7 +131,7 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
     if (*abort_flag) return false;
     const uint64_t now = ptx::globaltimer_ns();
     if (t0 == 0) t0 = now;
-    if (now - t0 > limit_ns) {
+    if (now - t0 > kWaitLimitNs) {
       *abort_flag = 1;
       atomicOr(status, MGF_DEV_WAIT_TIMEOUT);
       return false;
@@ -328,6 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* drain_bar = bars + 2 * STAGES + 2 * BUFS;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(drain_bar + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  drain::Copies* loads = reinterpret_cast<drain::Copies*>(tmem_holder + 2);  // the producer's, when it has stopped
   int* prefix = reinterpret_cast<int*>(smem + STAGES * C::STAGE_BYTES + C::BAR_BYTES);
   int* seg_start = prefix + (kMaxGroups + 1);
   int* seg_end = seg_start + (kMaxGroups + 1);
@@ -349,6 +350,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     ptx::mbar_init(ptx::smem_u32(drain_bar), 1);
     *abort_flag = 0;
+    *loads = drain::Copies();
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tmA);
     ptx::prefetch_tmap(&tmB);
@@ -381,9 +383,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ TMA producer
     if (ptx::elect_one()) {
       uint32_t stage = 0, phase = 0;
-      uint32_t issued = 0, issued_parity = 0;  // one bit per stage
+      drain::Copies armed;
       bool ok = true;
-      for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+      for (int t = unit; ok && t < total_tiles && p.stall_test != 1; t += num_units) {
         const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
         const int nb0 = ti.n0 + static_cast<int>(crank) * C::BNC;
         // a tile of up to 32 rows loads 32 rows of A; the products of the stage's other rows are never read
@@ -413,17 +415,11 @@ __global__ void __launch_bounds__(kThreads, 1)
               ptx::tma_load_3d(sB, &tmB, fb, kb * BK, nb0, ti.e);
             }
           }
-          issued |= 1u << stage;
-          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+          if (leader) armed.arm(stage, phase);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok && CG == 1) {
-        // Stopped early: let the copies in flight land before the CTA exits (a pair meets at its barrier).
-        for (int s = 0; s < STAGES; ++s)
-          if ((issued >> s) & 1u)
-            wait_bounded(ptx::smem_u32(&full_bar[s]), (issued_parity >> s) & 1u, abort_flag, p.status, kDrainLimitNs);
-      }
+      *loads = armed;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (one elected thread of the even CTA)
@@ -434,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
     constexpr uint32_t a_kstep = 32u >> 4;
     uint32_t stage = 0, phase = 0, part = 0;  // part: k blocks multiplied so far, the TMEM buffers in turn
-    bool ok = true, issued_any = false;
+    bool ok = p.stall_test != 2;
     if (leader && ptx::elect_one()) {
       for (int t = unit; ok && t < total_tiles; t += num_units) {
         for (int kb = 0; kb < nk; ++kb, ++part) {
@@ -461,15 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             ptx::umma_commit(ptx::smem_u32(&tfull_bar[buf]));
             ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
           }
-          issued_any = true;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
-      }
-      if (!ok && issued_any) {
-        // Stopped early: wait for the UMMAs already issued before TMEM is released.
-        if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
-        else ptx::umma_commit(ptx::smem_u32(drain_bar));
-        wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, p.status, kDrainLimitNs);
       }
     }
     __syncwarp();
@@ -533,6 +522,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   ptx::tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // stopped early: the same for all threads, every role has ended
+    if (warp == 0 && ptx::elect_one()) drain::copies<CG>(*loads, full_bar, p.status);
+    if (warp == 1 && leader && ptx::elect_one()) drain::products<CG>(drain_bar, p.status);
+    __syncthreads();
+  }
   // A pair leaves together: the peer may still signal this CTA's barriers until both are done.
   if constexpr (CG == 2) ptx::cluster_sync();
   if (warp == 1) {
@@ -644,6 +638,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
   uint64_t* drain_bar = tfull_bar + 2;
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(tfull_bar + 3);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
+  drain::Copies* loads = reinterpret_cast<drain::Copies*>(tmem_holder + 2);  // the producer's, when it has stopped
   int* prefix = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + C::BAR_BYTES);
   int* seg_start = prefix + (kMaxGroups + 1);
   int* seg_end = seg_start + (kMaxGroups + 1);
@@ -675,6 +670,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
     ptx::mbar_init(ptx::smem_u32(tempty_bar), kNumEpiWarps * CG);
     ptx::mbar_init(ptx::smem_u32(drain_bar), 1);
     *abort_flag = 0;
+    *loads = drain::Copies();
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tmA);
     ptx::prefetch_tmap(&tmB);
@@ -703,9 +699,9 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
     // ------------------------------------------------------------ TMA producer
     if (ptx::elect_one()) {
       uint32_t stage = 0, phase = 0;
-      uint32_t issued = 0, issued_parity = 0;  // one bit per stage
+      drain::Copies armed;
       bool ok = true;
-      for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+      for (int t = unit; ok && t < total_tiles && p.stall_test != 1; t += num_units) {
         const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
         // a tile of few rows loads 32 or 64 rows of A; the products of the stage's other rows are never read
         const int rows = CG == 2 || ti.row_end - ti.row0 > 64 ? BM : ti.row_end - ti.row0 > 32 ? 64 : 32;
@@ -734,16 +730,11 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
               ptx::tma_load_3d(sB, &tmB, fb, kb * BK, col, ti.e);
             }
           }
-          issued |= 1u << stage;
-          issued_parity = (issued_parity & ~(1u << stage)) | (phase << stage);
+          if (leader) armed.arm(stage, phase);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
       }
-      if (!ok && CG == 1) {  // stopped early: let the copies in flight land before the CTA exits (a pair meets below)
-        for (int s = 0; s < STAGES; ++s)
-          if ((issued >> s) & 1u)
-            wait_bounded(ptx::smem_u32(&full_bar[s]), (issued_parity >> s) & 1u, abort_flag, p.status, kDrainLimitNs);
-      }
+      *loads = armed;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (one elected thread of the even CTA)
@@ -752,7 +743,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
       constexpr uint32_t b_kstep = B_MN ? (32u * 128u) >> 4 : 32u >> 4;
       constexpr uint32_t a_kstep = 32u >> 4;
       uint32_t stage = 0, phase = 0, slot = 0, sphase = 0, tphase = 0;
-      bool ok = true, issued_any = false;
+      bool ok = p.stall_test != 2;
       for (int t = unit; ok && t < total_tiles; t += num_units, tphase ^= 1) {
         ok = wait_bounded(ptx::smem_u32(tempty_bar), tphase ^ 1, abort_flag, p.status);
         if (!ok) break;
@@ -787,7 +778,6 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
             else
               ptx::umma_mxf8(tmem_base, adesc + kk * a_kstep, bdesc + kk * b_kstep, idesc, sfa, sfb, (kb | kk) != 0);
           }
-          issued_any = true;
           commit(&empty_bar[stage]);
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
           if ((kb & 3) == 3 || kb == nk - 1) {
@@ -798,11 +788,6 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
         if (!ok) break;
         commit(tfull_bar);
       }
-      if (!ok && issued_any) {  // stopped early: wait for the UMMAs already issued before TMEM is released
-        if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
-        else ptx::umma_commit(ptx::smem_u32(drain_bar));
-        wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, p.status, kDrainLimitNs);
-      }
     }
     __syncwarp();
   } else if (warp == 2) {
@@ -811,7 +796,7 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
     // columns for B, which within one block of 128 are all the same word).
     uint32_t slot = 0, sphase = 0;
     bool ok = true;
-    for (int t = unit; ok && t < total_tiles && !p.stall_test; t += num_units) {
+    for (int t = unit; ok && t < total_tiles && p.stall_test != 1; t += num_units) {
       const Tile ti = decode_tile<TM, BN>(t, p, prefix, seg_start, seg_end);
       const uint32_t* pa = p.packed_a + ti.row0 + static_cast<int>(crank) * BM + lane;
       const int c0 = ti.n0 / BK, c1 = c0 + 1 < nnb ? c0 + 1 : c0;
@@ -871,6 +856,11 @@ __global__ void __launch_bounds__(MxCfg<CG>::kThreads, 1)
 
   ptx::tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // stopped early: the same for all threads, every role has ended
+    if (warp == 0 && ptx::elect_one()) drain::copies<CG>(*loads, full_bar, p.status);
+    if (warp == 1 && leader && ptx::elect_one()) drain::products<CG>(drain_bar, p.status);
+    __syncthreads();
+  }
   // A pair leaves together: the peer may still signal this CTA's barriers until both are done.
   if constexpr (CG == 2) ptx::cluster_sync();
   if (warp == 1) {
@@ -1092,7 +1082,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   if (p.status == nullptr) return MGF_ERR_CUDA;
   {
     const char* env = getenv("MGF_TEST_STALL_PRODUCER");  // see moe_gemm_sm100.cu
-    p.stall_test = (env != nullptr && env[0] == '1') ? 1 : 0;
+    p.stall_test = env != nullptr && (env[0] == '1' || env[0] == '2') ? env[0] - '0' : 0;
   }
 
   // Pairs (256-row tiles, half the B bytes per SM) for groups of 2048 rows and more on average (32 groups, k = 2880,

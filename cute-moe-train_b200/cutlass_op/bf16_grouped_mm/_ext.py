@@ -21,6 +21,7 @@ OPS_PATH = _HERE / "_grouped_mm_ops.so"
 DEV_WAIT_TIMEOUT = 0x1
 DEV_BAD_OFFS = 0x2
 DEV_ROW_OUT_OF_RANGE = 0x4
+DEV_DRAIN_TIMEOUT = 0x8
 
 
 def _require(path: Path) -> None:
@@ -92,6 +93,8 @@ def check_device_status(device: int | None = None) -> None:
         what = []
         if st & DEV_WAIT_TIMEOUT:
             what.append("a pipeline wait ran out and the kernel stopped early")
+        if st & DEV_DRAIN_TIMEOUT:
+            what.append("copies or products in flight did not end after that either")
         if st & DEV_BAD_OFFS:
             what.append("offs was not non-decreasing within [0, total rows]")
         if st & DEV_ROW_OUT_OF_RANGE:

@@ -54,6 +54,7 @@ enum mgf_status {
 
 /* Device status bits recorded by the kernels (read with mgf_device_status). */
 #define MGF_DEV_WAIT_TIMEOUT 0x1u  /* a pipeline wait ran out; the kernel stopped early        */
+#define MGF_DEV_DRAIN_TIMEOUT 0x8u /* after that, its own copies or products in flight did not end in time either */
 #define MGF_DEV_BAD_OFFS 0x2u      /* offs not non-decreasing or beyond the row extent; clamped */
 #define MGF_DEV_ROW_OUT_OF_RANGE 0x4u /* a row index of gather/combine/push/permute fell outside its buffer (or an expert id its range);
                                          that row was skipped (left unwritten)                    */
