@@ -40,6 +40,7 @@
 #include <cstdlib>
 #include <mutex>
 
+#include "drain.cuh"
 #include "epilogue.cuh"
 #include "host.h"
 #include "moe_gemm.h"
@@ -57,7 +58,6 @@ constexpr int kNumEpiWarps = 4 * kEpiGroups;
 constexpr int kThreads = 64 + 32 * kNumEpiWarps;
 constexpr int kRing = 4;                      // tile ids in flight between the producer and the consumers
 constexpr uint64_t kWaitLimitNs = 1500ull * 1000ull * 1000ull;  // 1.5 s per pipeline wait
-constexpr uint64_t kDrainLimitNs = 100ull * 1000ull * 1000ull;
 
 // OB: 2 KB output staging slices per epilogue warp (ragged-K TMA-store epilogue).  OB = 1: one
 // 32 x 32 store per chunk.  OB = 4 (short groups): a warp stages all its chunks of a tile (32 rows x
@@ -81,7 +81,7 @@ struct TileCfg {
   static constexpr int STAGES = (BUDGET / STAGE_BYTES) > 8 ? 8 : (BUDGET / STAGE_BYTES);
   static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + OUT_OFFSET + OUT_BYTES;
   static_assert(STAGES >= 3, "pipeline depth");
-  static_assert((3 * STAGES + 5 + 4 * kRing) * 8 + 8 + 8 * kRing <= BAR_BYTES, "barrier area");
+  static_assert((3 * STAGES + 5 + 4 * kRing) * 8 + 16 + 8 * kRing <= BAR_BYTES, "barrier area");
   static_assert(SMEM_BYTES <= 227 * 1024, "shared memory budget");
 };
 
@@ -113,7 +113,7 @@ struct Params {
   int store_aux;
   int aux_v8;         // aux base 32-byte aligned and row pitch a multiple of 32 bytes
   int d_v8, d2_v8;    // the same for the ragged-M outputs d and d2
-  int stall_test;     // test hook: the producer hands out no tiles, so every consumer wait runs out
+  int stall_test;     // test hook: 1: the producer hands out no tiles, 2: none is multiplied; every wait behind that runs out
   int* tile_counter;  // zero-filled device counter: dynamic tile order; nullptr = static striding
   const long long* d_rows;  // BIAS scatter mode: destination address of every output row (0 = none)
   int group_begin;          // ragged-M: groups below this index have no tiles (their rows are not touched)
@@ -141,11 +141,10 @@ __device__ __forceinline__ bool try_wait_sel(uint32_t bar, uint32_t parity) {
   return ptx::mbar_try_wait(bar, parity);
 }
 
-// Wait for phase `parity` of an mbarrier for at most `limit_ns`.  CLUSTER = true acquires at
+// Wait for phase `parity` of an mbarrier for at most kWaitLimitNs.  CLUSTER = true acquires at
 // cluster scope (barriers that the peer CTA of a pair also arrives on).
 template <bool CLUSTER = false>
-__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                             uint64_t limit_ns = kWaitLimitNs) {
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
   if (try_wait_sel<CLUSTER>(bar, parity)) return true;
   const uint64_t t0 = ptx::globaltimer_ns();
   uint32_t it = 0;
@@ -153,7 +152,7 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, vola
     if (try_wait_sel<CLUSTER>(bar, parity)) return true;
     if ((++it & 127u) == 0) {
       if (*abort_flag) return false;
-      if (ptx::globaltimer_ns() - t0 > limit_ns) {
+      if (ptx::globaltimer_ns() - t0 > kWaitLimitNs) {
         *abort_flag = 1;
         atomicOr(&g_status, MGF_DEV_WAIT_TIMEOUT);
         return false;
@@ -320,7 +319,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* mbox_empty = bars + 3 * STAGES + 5 + 3 * kRing;  // leader: the odd CTA took the id
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(bars + 3 * STAGES + 5 + 4 * kRing);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_holder + 1);
-  volatile int* ring_ids = reinterpret_cast<volatile int*>(tmem_holder + 2);
+  drain::Copies* loads = reinterpret_cast<drain::Copies*>(tmem_holder + 2);  // the producer's, when it has stopped
+  volatile int* ring_ids = reinterpret_cast<volatile int*>(tmem_holder + 4);
   volatile int* mbox_ids = ring_ids + kRing;
   int* sched = reinterpret_cast<int*>(smem + STAGES * Cfg::STAGE_BYTES + Cfg::BAR_BYTES);
   uint8_t* out_stage = smem + STAGES * Cfg::STAGE_BYTES + Cfg::OUT_OFFSET;  // 1024-aligned
@@ -351,6 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(ptx::smem_u32(&mbox_empty[j]), 1);
     }
     *abort_flag = 0;
+    *loads = drain::Copies();
     ptx::fence_mbar_init();
     ptx::prefetch_tmap(&tmA);
     ptx::prefetch_tmap(&tmB);
@@ -400,10 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       constexpr uint32_t kLoadBytes = Cfg::STAGE_BYTES;  // bytes landing in this CTA per stage
       uint32_t stage = 0, phase = 0;
-      uint32_t issued_parity[STAGES];
-      bool outstanding[STAGES];
-#pragma unroll
-      for (int s = 0; s < STAGES; ++s) { outstanding[s] = false; issued_parity[s] = 0; }
+      drain::Copies armed;      // stages whose copies count on this CTA's barrier
+      uint32_t own_phase = 0;   // odd CTA: per-stage phase of its own barrier, which relayed stages alone use
       bool ok = true;
       // The producer picks the tile sequence (static striding, or an atomic counter when the
       // launch has one) and hands every tile id to the MMA and epilogue warps through the ring.
@@ -413,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int t = unit;
       uint32_t rslot = 0, rphase = 0;
       uint32_t mslot = 0, mphase = 0;
-      while (ok && !p.stall_test) {
+      while (ok && p.stall_test != 1) {
         if (!wait_bounded(ptx::smem_u32(&ring_empty[rslot]), rphase ^ 1, abort_flag)) { ok = false; break; }
         if (forwarded) {
           if (leader) {
@@ -445,13 +444,17 @@ __global__ void __launch_bounds__(kThreads, 1)
             const bool relay = relayed(ti, kb, odd_ones);
             if (leader) {
               ptx::mbar_arrive_expect_tx(own_full, relay ? kLoadBytes : 2 * kLoadBytes);
+              armed.arm(stage, phase);
             } else if (relay) {
               ptx::mbar_arrive_expect_tx(own_full, kLoadBytes);
+              armed.arm(stage, (own_phase >> stage) & 1u);
+              own_phase ^= 1u << stage;
             } else {
               fb = leader_addr(&full_bar[stage]);
             }
           } else {
             ptx::mbar_arrive_expect_tx(own_full, kLoadBytes);
+            armed.arm(stage, phase);
           }
           const uint32_t sA = ptx::smem_u32(stage_base + stage * Cfg::STAGE_BYTES);
           const uint32_t sB = sA + Cfg::A_BYTES;
@@ -497,8 +500,6 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int c = 0; c < Cfg::B_CHUNKS; ++c) load2(sB + c * 8192, &tmB, nb0 + 64 * c, kr);
             }
           }
-          outstanding[stage] = true;
-          issued_parity[stage] = phase;
           if (++stage == STAGES) { stage = 0; phase ^= 1; }
         }
         // (claiming the next id at the start of the tile instead was measured: each CTA then holds two
@@ -507,12 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (p.tile_counter == nullptr) t += num_units;
         else if (leader) t = num_units + atomicAdd(p.tile_counter, 1);  // the odd CTA reads its mailbox
       }
-      if (!ok && CG == 1) {
-        // Stopped early: let the copies already in flight land before the CTA exits.  (A pair waits
-        // for its copies at the final cluster barrier.)
-        for (int s = 0; s < STAGES; ++s)
-          if (outstanding[s]) wait_bounded(ptx::smem_u32(&full_bar[s]), issued_parity[s], abort_flag, kDrainLimitNs);
-      }
+      *loads = armed;
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (even CTA) /
@@ -531,8 +527,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool issuer = (CG == 1) || leader;
     uint32_t stage = 0, phase = 0;
     uint32_t relay_bits = 0;  // per-stage phase of patch_done (even CTA) / own full (odd CTA) on relayed stages
-    bool ok = true;
-    bool issued_any = false;
+    bool ok = p.stall_test != 2;
     uint32_t rslot = 0, rphase = 0;
     for (int it = 0; ok; ++it) {
       ok = __all_sync(0xffffffffu, wait_bounded(ptx::smem_u32(&ring_full[rslot]), rphase, abort_flag));
@@ -639,7 +634,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(&empty_bar[stage]), 0x3);
           else ptx::umma_commit(ptx::smem_u32(&empty_bar[stage]));
-          issued_any = true;
         }
         __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1; }
@@ -657,13 +651,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       __syncwarp();
     }
-    if (!ok && issuer && lane == 0 && issued_any) {
-      // Stopped early: wait for the UMMAs already issued before TMEM is released.
-      if constexpr (CG == 2) ptx::umma_commit_pair(ptx::smem_u32(drain_bar), 0x1);
-      else ptx::umma_commit(ptx::smem_u32(drain_bar));
-      wait_bounded(ptx::smem_u32(drain_bar), 0, abort_flag, kDrainLimitNs);
-    }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ epilogue warps
     // Two warpgroups; each reads all 128 TMEM lanes (warp w owns lanes 32*(w%4)..+31, i.e. 32
@@ -969,6 +956,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   ptx::tc_fence_before();
   __syncthreads();
+  if (*abort_flag) {  // stopped early: the same for all threads, every role has ended
+    if (warp == 0 && lane == 0) drain::copies<CG>(*loads, full_bar, &g_status);
+    if (warp == 1 && leader && lane == 0) drain::products<CG>(drain_bar, &g_status);
+    __syncthreads();
+  }
   // A pair leaves together: the peer may still signal this CTA's barriers until both are done.
   if constexpr (CG == 2) ptx::cluster_sync();
   if (warp == 1) {
@@ -1494,11 +1486,12 @@ extern "C" int mgf_grouped_gemm_launch(const mgf_gemm_desc* desc, void* stream) 
   // sequence, which static striding gives them.
   p.tile_counter = (g.epilogue == MGF_EPI_WGRAD) ? g.workspace : nullptr;
   // Test hook for the bounded waits: with MGF_TEST_STALL_PRODUCER=1 the kernel does no work and
-  // every consumer wait gives up after its limit, setting MGF_DEV_WAIT_TIMEOUT.  Nothing is in flight
-  // when they give up, so the context stays usable; tests use it to exercise that path on a GPU.
+  // every consumer wait gives up after its limit, setting MGF_DEV_WAIT_TIMEOUT.  With 2 the producer
+  // loads and nothing is multiplied: the waits give up with every stage filled, and the kernel waits
+  // for those copies before it leaves.  The context stays usable; tests exercise these paths on a GPU.
   {
     const char* env = getenv("MGF_TEST_STALL_PRODUCER");
-    p.stall_test = (env != nullptr && env[0] == '1') ? 1 : 0;
+    p.stall_test = env != nullptr && (env[0] == '1' || env[0] == '2') ? env[0] - '0' : 0;
   }
   if (cg == 2) {
     switch (bn) {

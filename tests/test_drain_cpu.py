@@ -76,3 +76,11 @@ def test_kernels_drain_behind_their_roles_and_before_they_leave(name, kernel):
     assert "CG == 1" not in tail  # a pair drains too
     # no wait that looks at the abort flag has a limit of its own any more
     assert not re.search(r"wait_bounded\([^;]*kDrain", source)
+
+
+def test_the_bf16_kernel_drains_too():
+    source = (CSRC / "moe_gemm_sm100.cu").read_text()
+    tail = _tail(source, "grouped_gemm_kernel(const")
+    order = [tail.index(s) for s in ("drain::copies<CG>", "drain::products<CG>", "cluster_sync")]
+    assert order == sorted(order) and "CG == 1" not in tail
+    assert not re.search(r"wait_bounded\([^;]*kDrain", source)
