@@ -55,7 +55,7 @@ def _objects(srcs: list[Path], headers: list[Path], cmd: list, verbose: bool, fo
 
 
 def build_lib(verbose: bool = False, force: bool = False) -> Path:
-    headers = sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+    headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
     cmd = [NVCC, *ARCH_FLAGS, "-O3", "-lineinfo", "-std=c++17", "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC",
            f"-I{INCLUDE}", f"-I{CSRC}"]
     objs = _objects(sorted(CSRC.glob("*.cu")), headers, cmd, verbose, force)
