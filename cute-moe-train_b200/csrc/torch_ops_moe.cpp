@@ -505,9 +505,11 @@ void no_tangent(const Tensor& t, const char* what) {
 
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
-// A gradient as the kernels take it: unit stride along the last dimension, rows apart.
+// A gradient as the kernels take it: unit stride along the last dimension, rows apart (a broadcast gradient of one
+// column has rows of one element at stride 0).
 Tensor row_major(const Tensor& g) {
-  return g.size(1) > 1 && (g.stride(1) != 1 || (g.size(0) > 1 && g.stride(0) < g.size(1))) ? g.contiguous() : g;
+  const bool dense = g.size(1) <= 1 || g.stride(1) == 1, apart = g.size(0) <= 1 || g.stride(0) >= g.size(1);
+  return dense && apart ? g : g.contiguous();
 }
 
 // The backward passes are kernels without a derivative of their own: create_graph is refused, not ignored.
