@@ -1145,8 +1145,9 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
       return MGF_ERR_CUDA;
     const int64_t mx_tiles = (g.total_rows / (BM * mx_cg) + g.num_groups) * static_cast<int64_t>(pm.n_tiles);
     if (mx_tiles > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
-    const int rc = mx_cg == 2 ? dispatch_mx<2>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, sms, st)
-                              : dispatch_mx<1>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, sms, st);
+    const int mx_sms = std::max(sms, mx_cg);  // a pair needs two
+    const int rc = mx_cg == 2 ? dispatch_mx<2>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, mx_sms, st)
+                              : dispatch_mx<1>(g.epilogue, b_mn, tA, tA32, tA64, tBm, pm, mx_tiles, mx_sms, st);
     if (rc != MGF_OK) return rc;
   }
   if (bn == 128) return dispatch<128, 1>(g.epilogue, b_mn, tA, tA32, tB, p, tiles, sms, st);

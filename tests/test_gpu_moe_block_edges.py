@@ -30,3 +30,27 @@ def test_gradients_of_rows_of_one_element_broadcast_over_the_tokens(T, k, dtype)
     c = plan.copy_of_row.long()
     assert torch.equal(y.grad.flatten(), w.detach().flatten()[c].to(dtype))
     assert torch.equal(w.grad.flatten()[c], y.detach().flatten().float())
+
+
+@pytest.mark.parametrize("sms_left", [1, 2, 3])
+@pytest.mark.parametrize("rows", [1100, 3000])
+def test_products_on_the_few_sms_that_a_carve_out_leaves(rows, sms_left, monkeypatch):
+    from cutlass_op.bf16_grouped_mm import fp8_block
+
+    monkeypatch.setenv("MGF_BLOCK_MX", "1")
+    for name in ("MGF_CTA_GROUP", "MGF_BN"):
+        monkeypatch.delenv(name, raising=False)
+    g = _gen(rows)
+    x = torch.randn(rows, 256, generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randn(1, 256, 512, generator=g, device="cuda").to(torch.bfloat16)
+    offs = torch.tensor([rows], dtype=torch.int32, device="cuda")
+    qa, sa = fp8_block.quantize_rows_block(x)
+    qb, sb = fp8_block.quantize_weights_block(w)
+    want = fp8_block.grouped_mm_fp8_block(qa, qb, offs, sa, sb)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    torch._C._set_sm_carveout_experimental(sms - sms_left)
+    try:
+        got = fp8_block.grouped_mm_fp8_block(qa, qb, offs, sa, sb)
+    finally:
+        torch._C._set_sm_carveout_experimental(None)
+    assert torch.equal(got, want)
