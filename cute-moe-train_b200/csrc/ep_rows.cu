@@ -15,6 +15,7 @@
 #include <cstdint>
 #include <cstring>
 
+#include "host.h"
 #include "moe_gemm.h"
 
 namespace mgf {
@@ -227,6 +228,7 @@ extern "C" int mgf_gather_rows(const void* src, int64_t ld_src, int64_t n_src, c
                                const float* scale, int64_t n_rows, int64_t row_elems, void* dst, int64_t ld_dst,
                                void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (n_rows < 0 || row_elems < 0 || n_src < 0) return MGF_ERR_INVALID_ARGUMENT;
   if (n_rows == 0 || row_elems == 0) return MGF_OK;
   if (src == nullptr || idx == nullptr || dst == nullptr) return MGF_ERR_INVALID_ARGUMENT;
@@ -243,6 +245,7 @@ extern "C" int mgf_combine_rows(const void* rows, int64_t ld_rows, int64_t n_row
                                 const float* weights, int64_t n_out, int32_t k, int64_t row_elems, void* out,
                                 int64_t ld_out, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (n_out < 0 || row_elems < 0 || k < 0 || n_rows < 0) return MGF_ERR_INVALID_ARGUMENT;
   if (n_out == 0 || row_elems == 0) return MGF_OK;
   if (out == nullptr || (k > 0 && (rows == nullptr || pos == nullptr))) return MGF_ERR_INVALID_ARGUMENT;
@@ -262,6 +265,7 @@ extern "C" int mgf_push_rows(const void* src, int64_t ld_src, int64_t n_src, con
                              unsigned long long* counter, unsigned long long seq, int64_t rank,
                              const int64_t* rotate, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (n_max < 0 || row_elems < 0 || n_src < 0) return MGF_ERR_INVALID_ARGUMENT;
   if (flag_bases != nullptr && (counter == nullptr || rank < 0 || rank >= world)) return MGF_ERR_INVALID_ARGUMENT;
   const PushSignal sig{flag_bases, counter, seq, rank};
@@ -325,6 +329,7 @@ extern "C" int mgf_ipc_close(void* base) {
 extern "C" int mgf_wait_flags(const unsigned long long* flags, int64_t world, unsigned long long seq,
                               int64_t timeout_ns, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (flags == nullptr || world <= 0 || world > 1024 || timeout_ns <= 0) return MGF_ERR_INVALID_ARGUMENT;
   unsigned int* status = status_word_address();
   if (status == nullptr) return MGF_ERR_CUDA;
@@ -552,6 +557,7 @@ extern "C" int mgf_ep_sort(const int64_t* expert_ids, int64_t n, int32_t num_exp
                            int32_t* workspace, int64_t* order, int64_t* inv_order, int64_t* copy_token,
                            int64_t* e_sorted, int64_t* counts, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (n < 0 || n > INT32_MAX || num_experts < 1 || num_experts > 1024 || topk < 1) return MGF_ERR_INVALID_ARGUMENT;
   if (counts == nullptr || workspace == nullptr ||
       (n > 0 && (expert_ids == nullptr || order == nullptr || inv_order == nullptr || copy_token == nullptr ||
@@ -583,6 +589,7 @@ extern "C" int mgf_ep_routes(const int64_t* c_all, int32_t world, int32_t num_ex
                              int64_t* dst_rank, int64_t* dst_row, int64_t* src_rank, int64_t* src_pos,
                              int64_t* ptr_ret, int64_t* ptr_gret, int32_t* offs, int32_t* n_recv, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (world < 1 || num_experts < 1 || num_experts % world || rank < 0 || rank >= world || n < 0 || cap < 1 ||
       n > INT32_MAX || cap > INT32_MAX || c_all == nullptr || workspace == nullptr || offs == nullptr ||
       n_recv == nullptr || src_rank == nullptr || src_pos == nullptr ||
@@ -606,6 +613,7 @@ extern "C" int mgf_ep_routes(const int64_t* c_all, int32_t world, int32_t num_ex
 extern "C" int mgf_signal_flags(const unsigned long long* flag_bases, int64_t world, int64_t rank,
                                 unsigned long long seq, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (flag_bases == nullptr || world < 1 || world > 1024 || rank < 0 || rank >= world) return MGF_ERR_INVALID_ARGUMENT;
   signal_flags_kernel<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(flag_bases, world, rank, seq);
   return cudaGetLastError() == cudaSuccess ? MGF_OK : MGF_ERR_CUDA;

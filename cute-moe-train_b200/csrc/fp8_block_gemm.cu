@@ -913,7 +913,7 @@ int launch_persistent(int threads, int smem, const char* form, int epi, bool b_m
   if (units > max_units[dev]) units = max_units[dev];
   if (tiles < units) units = static_cast<int>(tiles);
   cfg.gridDim = dim3(static_cast<unsigned>(units * CG));
-  cudaGetLastError();
+  forget_cuda_error();
   cudaError_t e = cudaLaunchKernelEx(&cfg, KERN, args...);
   if (e == cudaSuccess && debug_sync()) {
     e = cudaStreamSynchronize(st);
@@ -1132,6 +1132,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
     p.packed_rows = sp.rows;
     p.other_scales = words;
     p.num_words = kPackBlocks;
+    forget_cuda_error();
     pack_scales_kernel<<<kPackBlocks, 256, 0, st>>>(p, ws, ws + sp.a_words, words);
     if (cudaGetLastError() != cudaSuccess) return MGF_ERR_CUDA;
     Params pm = p;

@@ -20,6 +20,7 @@
 
 #include <cstdint>
 
+#include "host.h"
 #include "moe_gemm.h"
 
 namespace mgf {
@@ -240,6 +241,7 @@ extern "C" int mgf_fp8_block_quantize_rows(const void* x, int64_t ldx, int64_t t
                                            const int32_t* row_of_copy, const int32_t* offs_end, void* q, int64_t ldq,
                                            float* scale, int64_t lds, int64_t n_rows, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (tokens < 0 || cols < 0 || topk < 1 || n_rows < 0 || n_rows > INT32_MAX || tokens > INT32_MAX / topk)
     return MGF_ERR_INVALID_ARGUMENT;
   if (row_of_copy == nullptr && (topk != 1 || n_rows != tokens || offs_end != nullptr)) return MGF_ERR_INVALID_ARGUMENT;
@@ -263,6 +265,7 @@ extern "C" int mgf_fp8_block_quantize_weights(const void* w, int64_t E, int64_t 
                                               void* q, int64_t q_e, int64_t q_r, float* scale, int64_t ss_e,
                                               int64_t ss_r, int64_t ss_c, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (E < 0 || R < 0 || C < 0 || E > 65535 || R > 65535ll * kBlock || C > int64_t(INT32_MAX) * kBlock)
     return MGF_ERR_INVALID_ARGUMENT;
   if (E == 0 || R == 0 || C == 0) return MGF_OK;

@@ -23,6 +23,7 @@
 
 #include <cstdint>
 
+#include "host.h"
 #include "moe_gemm.h"
 
 namespace mgf {
@@ -490,6 +491,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 extern "C" int mgf_fp8_quantize_rows(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                                      float* scale, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (rows < 0 || cols < 0 || (rows > 0 && (x == nullptr || q == nullptr || scale == nullptr)))
     return MGF_ERR_INVALID_ARGUMENT;
   if (rows == 0) return MGF_OK;
@@ -503,6 +505,7 @@ extern "C" int mgf_fp8_quantize_rows(const void* x, int64_t rows, int64_t cols, 
 extern "C" int mgf_fp8_quantize_cols(const void* x, int64_t rows, int64_t cols, int64_t ldx, void* q, int64_t ldq,
                                      float* scale, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (rows < 0 || cols < 0 || (cols > 0 && scale == nullptr) || (rows > 0 && (x == nullptr || q == nullptr)))
     return MGF_ERR_INVALID_ARGUMENT;
   if (cols == 0) return MGF_OK;
@@ -527,6 +530,7 @@ extern "C" int mgf_fp8_quantize_cols(const void* x, int64_t rows, int64_t cols, 
 extern "C" int mgf_fp8_quantize_weights(const void* w, int64_t E, int64_t K, int64_t N, int64_t s_e, int64_t s_k,
                                         int64_t s_n, void* q, int64_t ldq, float* scale, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (E < 0 || K < 0 || N < 0 || ldq < K) return MGF_ERR_INVALID_ARGUMENT;
   if (E == 0 || N == 0) return MGF_OK;
   if (w == nullptr || q == nullptr || scale == nullptr) return MGF_ERR_INVALID_ARGUMENT;
@@ -563,6 +567,7 @@ extern "C" int mgf_fp8_quantize_weights_both(const void* w, int64_t E, int64_t K
                                              void* qa, int64_t ldqa, float* sa, void* qb, int64_t ldqb, float* sb,
                                              void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (E < 0 || K < 0 || N < 0 || ldqa < K || ldqb < N) return MGF_ERR_INVALID_ARGUMENT;
   if (E == 0) return MGF_OK;
   if (w == nullptr || qa == nullptr || qb == nullptr || sa == nullptr || sb == nullptr) return MGF_ERR_INVALID_ARGUMENT;
@@ -593,6 +598,7 @@ extern "C" int mgf_fp8_quantize_rows_cols(const void* x, int64_t rows, int64_t c
                                           int64_t ldq_r, float* s_r, void* q_c, int64_t ldq_c, float* s_c,
                                           void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (rows < 0 || cols < 0 || (cols > 0 && s_c == nullptr) || (rows > 0 && (s_r == nullptr)) ||
       (rows > 0 && cols > 0 && (x == nullptr || q_r == nullptr || q_c == nullptr)))
     return MGF_ERR_INVALID_ARGUMENT;

@@ -24,6 +24,10 @@ bool encode_bf16(CUtensorMap* m, const void* base, int rank, const uint64_t* dim
 void clear_error();
 void record_error(const char* what, cudaError_t e);
 
+// Called before a launch whose status is read with cudaGetLastError: an error that an unrelated runtime call left would
+// otherwise be reported as the launch's.
+inline void forget_cuda_error() { cudaGetLastError(); }
+
 bool bind_device(int dev);  // a current driver context for this host thread
 bool debug_sync();          // MGF_DEBUG_SYNC=1
 

@@ -19,6 +19,7 @@
 #include <cstdint>
 #include <type_traits>
 
+#include "host.h"
 #include "moe_gemm.h"
 
 namespace mgf {
@@ -625,6 +626,7 @@ extern "C" int64_t mgf_moe_sort_workspace_words(int64_t n, int32_t num_experts) 
 extern "C" int mgf_moe_sort(const int64_t* expert_idx, int64_t n, int32_t num_experts, int32_t* offs,
                             int32_t* row_of_copy, int32_t* copy_of_row, int32_t* workspace, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (n < 0 || n > INT32_MAX || num_experts < 1 || num_experts > 1024 || offs == nullptr)
     return MGF_ERR_INVALID_ARGUMENT;
   if (n > 0 && (expert_idx == nullptr || row_of_copy == nullptr || copy_of_row == nullptr))
@@ -661,6 +663,7 @@ extern "C" int mgf_moe_sort_permute(const int64_t* expert_idx, int32_t num_exper
                                     int32_t* row_of_copy, int32_t* copy_of_row, void* rows, int64_t ldr,
                                     int32_t* workspace, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (topk < 1 || tokens < 0 || tokens > INT32_MAX / topk) return MGF_ERR_INVALID_ARGUMENT;
   const int64_t n = tokens * topk;
   if (n == 0 || hidden == 0 || n > kFewCopies) {
@@ -705,6 +708,7 @@ extern "C" int mgf_moe_permute(const void* x, int32_t dtype, int64_t ldx, int64_
                                const int32_t* row_of_copy, const int32_t* offs_end, void* rows, int64_t ldr,
                                int64_t n_rows, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
   if (n_rows == 0 || hidden == 0) return MGF_OK;
   if (offs_end == nullptr || rows == nullptr || (tokens > 0 && (x == nullptr || row_of_copy == nullptr)))
@@ -730,6 +734,7 @@ extern "C" int mgf_moe_unpermute(const void* rows, int32_t dtype, int64_t ldr, i
                                  int32_t topk, int64_t hidden, const int32_t* row_of_copy, const float* weights,
                                  void* out, int64_t ldo, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
   if (tokens == 0 || hidden == 0) return MGF_OK;
   if (out == nullptr || row_of_copy == nullptr || (n_rows > 0 && rows == nullptr)) return MGF_ERR_INVALID_ARGUMENT;
@@ -757,6 +762,7 @@ extern "C" int mgf_moe_unpermute_bwd(const void* grad_out, int64_t ldg, const vo
                                      const int32_t* row_of_copy, const int32_t* offs_end, const float* weights,
                                      void* grad_rows, int64_t ldgr, float* grad_weights, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   if (!row_args_ok(dtype, tokens, topk, hidden, n_rows)) return MGF_ERR_INVALID_ARGUMENT;
   if (grad_rows == nullptr && grad_weights == nullptr) return MGF_OK;
   if (tokens > 0 && (grad_out == nullptr || row_of_copy == nullptr)) return MGF_ERR_INVALID_ARGUMENT;

@@ -24,6 +24,7 @@
 
 #include <cstdint>
 
+#include "host.h"
 #include "moe_gemm.h"
 
 namespace mgf {
@@ -247,6 +248,7 @@ extern "C" int mgf_moe_route(const void* logits, int32_t dtype, int64_t ld, int6
                              int32_t topk, int32_t score, int32_t renormalize, float scale, const float* bias,
                              const uint8_t* token_mask, float* weights, int64_t* expert_idx, void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   const bool on_score = (score & MGF_ROUTE_BIAS_ON_SCORE) != 0 && bias != nullptr;
   score &= ~MGF_ROUTE_BIAS_ON_SCORE;
   if (!route_args_ok(dtype, tokens, num_experts, topk, score)) return MGF_ERR_INVALID_ARGUMENT;
@@ -275,6 +277,7 @@ extern "C" int mgf_moe_route_bwd(const void* logits, int32_t dtype, int64_t ld, 
                                  const int64_t* expert_idx, const float* grad_weights, void* grad_logits, int64_t ldg,
                                  void* stream) {
   using namespace mgf;
+  forget_cuda_error();
   score &= ~MGF_ROUTE_BIAS_ON_SCORE;  // the bias is not in the weights
   if (!route_args_ok(dtype, tokens, num_experts, topk, score)) return MGF_ERR_INVALID_ARGUMENT;
   if (tokens == 0) return MGF_OK;
