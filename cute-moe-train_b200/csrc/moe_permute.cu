@@ -77,7 +77,7 @@ __device__ __host__ __forceinline__ int64_t copies_per_cta(int64_t n, int ctas) 
 // counts[cta][e] of every CTA's copies.
 __global__ void __launch_bounds__(256) count_kernel(const int64_t* __restrict__ ids, int64_t n, int E,
                                                     int32_t* __restrict__ counts) {
-  extern __shared__ int32_t smem[];
+  extern __shared__ __align__(16) int32_t smem[];
   for (int e = threadIdx.x; e < E; e += blockDim.x) smem[e] = 0;
   __syncthreads();
   const int64_t per = copies_per_cta(n, gridDim.x), begin = blockIdx.x * per;
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(1024) sort_kernel(const int64_t* __restrict__ 
                                                     int32_t* __restrict__ row_of_copy,
                                                     int32_t* __restrict__ copy_of_row,
                                                     unsigned int* __restrict__ status) {
-  extern __shared__ int32_t smem[];
+  extern __shared__ __align__(16) int32_t smem[];
   sort_copies<true>(smem, blockIdx.x, gridDim.x, ids, n, E, counts, offs, row_of_copy, copy_of_row, nullptr, status);
 }
 
@@ -407,7 +407,7 @@ __global__ void __launch_bounds__(1024)
                         int32_t* __restrict__ copy_of_row, T* __restrict__ rows, int64_t ldr,
                         unsigned int* __restrict__ status) {
   using A = Access<T, VEC>;
-  extern __shared__ int32_t smem[];
+  extern __shared__ __align__(16) int32_t smem[];
   const int lane = threadIdx.x & 31, warps = blockDim.x >> 5;
   const int64_t n = tokens * topk;
   int32_t* row_of = smem + (n <= kCountedCopies ? kCountedCopies : (warps + 2) * E);
