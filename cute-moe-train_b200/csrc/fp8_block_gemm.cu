@@ -1028,7 +1028,7 @@ extern "C" int mgf_block_gemm_launch(const mgf_block_gemm_desc* desc, void* stre
   const mgf_block_gemm_desc& g = *desc;
   if (g.num_groups < 1 || g.num_groups > kMaxGroups) return MGF_ERR_TOO_MANY_GROUPS;
   if (g.epilogue < MGF_EPI_BIAS || g.epilogue > MGF_EPI_SWIGLU_BWD) return MGF_ERR_INVALID_ARGUMENT;
-  if (g.total_rows < 0 || g.total_rows > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.total_rows < 0 || g.total_rows > kMaxRows) return MGF_ERR_INVALID_ARGUMENT;
   if (g.n <= 0 || g.k <= 0 || g.n > INT32_MAX / 2 || g.k > INT32_MAX / 2 || g.n % 8 != 0) return MGF_ERR_INVALID_ARGUMENT;
   if (g.epilogue == MGF_EPI_SWIGLU && g.n % 16 != 0) return MGF_ERR_INVALID_ARGUMENT;
   if (g.total_rows == 0) return MGF_OK;  // nothing to write; the tensors of an empty batch have no address

@@ -8,6 +8,9 @@
 
 namespace mgf {
 
+// Rows of a product: a tile's row index, up to 256 past the last row, is a 32-bit number.
+constexpr int64_t kMaxRows = INT32_MAX - 256;
+
 struct DeviceInfo {
   int sms = 0;
   int major = 0;

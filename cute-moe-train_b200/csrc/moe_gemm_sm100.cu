@@ -1261,7 +1261,7 @@ extern "C" int mgf_grouped_gemm_launch(const mgf_gemm_desc* desc, void* stream) 
   const mgf_gemm_desc& g = *desc;
   if (g.num_groups < 1 || g.num_groups > kMaxGroups) return MGF_ERR_TOO_MANY_GROUPS;
   if (g.epilogue < MGF_EPI_BIAS || g.epilogue > MGF_EPI_WGRAD) return MGF_ERR_INVALID_ARGUMENT;
-  if (g.total_rows < 0 || g.total_rows > INT32_MAX) return MGF_ERR_INVALID_ARGUMENT;
+  if (g.total_rows < 0 || g.total_rows > kMaxRows) return MGF_ERR_INVALID_ARGUMENT;
   const bool ragged_k = g.epilogue == MGF_EPI_WGRAD;
   // Ragged-M with no rows has nothing to write.  Ragged-K with no rows still writes zeros for
   // every group (A and B, possibly NULL, are then never read).

@@ -83,7 +83,7 @@ enum mgf_status {
 typedef struct mgf_gemm_desc {
   int32_t epilogue;      /* enum mgf_epilogue */
   int32_t num_groups;    /* E (1..1024) */
-  int64_t total_rows;    /* extent of the ragged dimension (tokens) */
+  int64_t total_rows;    /* extent of the ragged dimension (tokens), at most 2^31 - 257 */
   int64_t m, n, k;       /* fixed GEMM extents (m unused for ragged-M, k unused for ragged-K) */
   const void* a;
   int64_t lda;
@@ -333,7 +333,7 @@ int mgf_fp8_block_quantize_weights(const void* w, int64_t E, int64_t R, int64_t 
 typedef struct mgf_block_gemm_desc {
   int32_t epilogue;
   int32_t num_groups;
-  int64_t total_rows, n, k;
+  int64_t total_rows, n, k; /* total_rows at most 2^31 - 257 */
   const void* a;
   int64_t lda;
   const void* b;
