@@ -16,7 +16,9 @@
 //                 groups, n = 5760, k = 2880.  Few rows: the weights' bytes.
 //   mx_kernel     powers of two.  The tensor cores apply the scales and the accumulator stays in TMEM: 2.3 PFLOP/s at the
 //                 same sizes, bound by the products' issue and shared-memory traffic (operands written and read) and,
-//                 sustained, by the power cap.  128 rows over 256 experts, n = 4096, k = 7168: 250 us, 5.9 TB/s of weights.
+//                 sustained, by the power cap: 98304 x 2880 x 5760 with SwiGLU over 32 experts 1480 us in short bursts,
+//                 1680-1740 back to back (1.9 PFLOP/s), as long as with one scale per row in the same run.  128 rows over
+//                 256 experts, n = 4096, k = 7168: 250 us, 5.9 TB/s of weights.
 //
 // B is read as stored, [E, k, n] with unit stride along n (the weights' own layout: MN-major operand) or along
 // k (the transposed view, the input gradient), so one set of codes serves both.  Warp roles, CTA pairs,
@@ -999,7 +1001,8 @@ int64_t wide_tiles(const mgf_block_gemm_desc& g) {
 // waits for (8 groups, k = n = 2048: 25 against 19 us at 1024 rows and 14 blocks, 33 against 43 at 4096 rows and 35);
 // from 120 on with few, where both forms wait for the weights and this one keeps more of them under way (128 rows,
 // k = 2880, n = 5760: 32 groups and 118 blocks 82 against 81, 128 groups and 460 blocks 126 against 137; 256 groups,
-// k = 2048, n = 7168: 127 against 136).  MGF_BLOCK_MX=0|1 forces a choice.
+// k = 2048, n = 7168: 127 against 136).  Rows behind the last group count as rows: how many they are is known on the device only.
+// MGF_BLOCK_MX=0|1 forces a choice.
 bool use_mx(const mgf_block_gemm_desc& g, int sms) {
   if (const char* env = getenv("MGF_BLOCK_MX"); env != nullptr && (env[0] == '0' || env[0] == '1')) return env[0] == '1';
   const int64_t blocks = wide_tiles(g) * ((g.k + BK - 1) / BK);

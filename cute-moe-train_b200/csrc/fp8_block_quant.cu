@@ -13,7 +13,8 @@
 //            codes is the forward's operand (unit stride along n) and, transposed, the input gradient's
 //            (unit stride along its k).
 // One read and one write each, bound by HBM: the block is held in registers between its maximum and its
-// codes.  Weights 32 x 2880 x 5760: 240 us, 6.6 TB/s; 8192 tokens x 7168 to 65536 rows: 97 us, 6.2 TB/s.
+// codes.  Weights 32 x 2880 x 5760: 248-262 us in calls back to back, 6.1-6.4 TB/s (240 in a loop of its own); 8192
+// tokens x 7168 to 65536 rows: 97 us, 6.2 TB/s; 98304 x 2880 without a plan 279 us, 3.0 TB/s (short-lived warps).
 #include <cuda_bf16.h>
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>

@@ -322,7 +322,8 @@ int mgf_fp8_block_quantize_weights(const void* w, int64_t E, int64_t R, int64_t 
 /* Grouped GEMM of e4m3 operands with a scale per block of 128 (ragged M; epilogues BIAS, SWIGLU and
  * SWIGLU_BWD, the fields that mgf_gemm_desc has too as there):
  *   acc[r, c] = sum_b scale_a[r, b] * scale_b[e, b, c / 128] * sum_{k in block b} a[r, k] * b[e, k, c]
- * with fp32 accumulation of every block and of their sum.  Any fp32 scales, not only powers of two.
+ * with fp32 accumulation of every block and of their sum.  Any fp32 scales, not only powers of two, whose products
+ * scale_a * scale_b are 0 or normal fp32 numbers.  NaN is kept, in the clamps of the SwiGLU too.
  *   a       e4m3 [total_rows, k], unit stride along k, row stride lda (bytes, a multiple of 16)
  *   b       e4m3 [E, k, n]: b_mn_major 1: unit stride along n, ldb between k rows; 0: unit stride along k, ldb
  *           between columns (bytes, multiples of 16; ldb_batch between groups likewise)
